@@ -61,6 +61,10 @@ EXPORTED = (
     "dta_check_workspace",
     "dta_backward_workspace_size",
     "dta_backward",
+    "dta_cache_write",
+    "dta_cache_read",
+    "dta_cache_decode_workspace_size",
+    "dta_cache_decode",
 )
 
 c_i32 = ctypes.c_int32
@@ -142,6 +146,52 @@ class BackwardArgs(ctypes.Structure):
     ]
 
 
+# dta_cache_format
+CACHE_FORMATS = {"e4m3": 0, "int8": 1}
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("n_kv_heads", c_i32), ("capacity", c_i32), ("head_dim", c_i32),
+        ("block", c_i32), ("format", c_i32),
+        ("k", c_vp), ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_s", c_i64),
+        ("v", c_vp), ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_s", c_i64),
+        ("k_scale", c_vp), ("k_scale_stride_b", c_i64), ("k_scale_stride_h", c_i64),
+        ("v_scale", c_vp), ("v_scale_stride_b", c_i64), ("v_scale_stride_h", c_i64),
+    ]
+
+
+class CacheWriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("n_new", c_i32), ("src_type", c_i32), ("pos", c_i32),
+        ("cache", CacheDesc),
+        ("k_new", c_vp), ("k_new_stride_b", c_i64), ("k_new_stride_h", c_i64), ("k_new_stride_s", c_i64),
+        ("v_new", c_vp), ("v_new_stride_b", c_i64), ("v_new_stride_h", c_i64), ("v_new_stride_s", c_i64),
+        ("pos_dev", c_vp), ("n_pos", c_i32), ("n_lengths", c_i32), ("lengths", c_vp),
+        ("error_word", c_vp),
+    ]
+
+
+class CacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("start", c_i32), ("n_keys", c_i32), ("dst_type", c_i32),
+        ("cache", CacheDesc),
+        ("out_k", c_vp), ("out_v", c_vp), ("lengths", c_vp), ("n_lengths", c_i32),
+    ]
+
+
+class CacheDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("n_heads", c_i32), ("n_keys", c_i32), ("window", c_i32), ("sink", c_i32),
+        ("scaling", ctypes.c_float),
+        ("cache", CacheDesc),
+        ("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64),
+        ("dense_out", c_vp), ("sparse_out", c_vp),
+        ("n_keys_dev", c_vp), ("n_lengths", c_i32),
+        ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class DtaError(RuntimeError):
     """Raised for any non-zero dta_status returned by the library."""
 
@@ -194,6 +244,14 @@ def lib() -> ctypes.CDLL:
         L.dta_backward_workspace_size.restype = ctypes.c_size_t
         L.dta_backward.argtypes = [ctypes.POINTER(BackwardArgs), c_vp]
         L.dta_backward.restype = ctypes.c_int
+        L.dta_cache_write.argtypes = [ctypes.POINTER(CacheWriteArgs), c_vp]
+        L.dta_cache_write.restype = ctypes.c_int
+        L.dta_cache_read.argtypes = [ctypes.POINTER(CacheReadArgs), c_vp]
+        L.dta_cache_read.restype = ctypes.c_int
+        L.dta_cache_decode_workspace_size.argtypes = [ctypes.POINTER(CacheDecodeArgs)]
+        L.dta_cache_decode_workspace_size.restype = ctypes.c_size_t
+        L.dta_cache_decode.argtypes = [ctypes.POINTER(CacheDecodeArgs), c_vp]
+        L.dta_cache_decode.restype = ctypes.c_int
         if L.dta_abi_version() != ABI_VERSION:
             raise RuntimeError("delta_attention_b200 library ABI mismatch")
         _lib = L

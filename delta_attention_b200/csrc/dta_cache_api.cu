@@ -1,0 +1,186 @@
+// extern "C" entry points of the 8-bit KV cache: argument validation, the
+// split of a decode call into chunks, and the launches.
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "delta_attention_b200.h"
+#include "dta_cache.h"
+#include "dta_internal.h"
+
+namespace {
+
+inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline bool stride16(long long s, int bytes) { return s > 0 && (s * bytes) % 16 == 0; }
+inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// Shapes, strides and pointers of a cache; *log_block and the two sides.
+int check_cache(const dta_cache_desc& c, int* log_block, dta::CacheSide side[2]) {
+  if (c.batch <= 0 || c.n_kv_heads <= 0 || c.capacity <= 0 || c.capacity > (1 << 30)) return DTA_ERR_SHAPE;
+  if (c.head_dim != 64 && c.head_dim != 128) return DTA_ERR_HEAD_DIM;
+  // the kernels' grid y is batch x KV head (at most 65535)
+  if ((long long)c.batch * c.n_kv_heads > 65535) return DTA_ERR_SHAPE;
+  if (c.block != 16 && c.block != 32 && c.block != 64 && c.block != 128) return DTA_ERR_INVALID_ARG;
+  if (c.format != DTA_CACHE_E4M3 && c.format != DTA_CACHE_INT8) return DTA_ERR_INVALID_ARG;
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale) return DTA_ERR_INVALID_ARG;
+  if (!aligned(c.k, 16) || !aligned(c.v, 16)) return DTA_ERR_ALIGNMENT;
+  for (long long s : {(long long)c.k_stride_b, (long long)c.k_stride_h, (long long)c.k_stride_s,
+                      (long long)c.v_stride_b, (long long)c.v_stride_h, (long long)c.v_stride_s})
+    if (!stride16(s, 1)) return DTA_ERR_STRIDE;
+  for (long long s : {(long long)c.k_scale_stride_b, (long long)c.k_scale_stride_h, (long long)c.v_scale_stride_b,
+                      (long long)c.v_scale_stride_h})
+    if (s <= 0) return DTA_ERR_STRIDE;
+  *log_block = c.block == 16 ? 4 : c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
+  side[0] = {reinterpret_cast<uint8_t*>(c.k), c.k_stride_b, c.k_stride_h, c.k_stride_s, c.k_scale,
+             c.k_scale_stride_b, c.k_scale_stride_h};
+  side[1] = {reinterpret_cast<uint8_t*>(c.v), c.v_stride_b, c.v_stride_h, c.v_stride_s, c.v_scale,
+             c.v_scale_stride_b, c.v_scale_stride_h};
+  return DTA_OK;
+}
+
+bool type_ok(int t) { return t == DTA_CACHE_BF16 || t == DTA_CACHE_FP16 || t == DTA_CACHE_FP32; }
+
+// An optional device list of one element or one per sequence; *step its stride.
+int check_list(const int32_t* list, int n, int batch, int* step) {
+  *step = 0;
+  if (!list) return DTA_OK;
+  if (!aligned(list, 4)) return DTA_ERR_ALIGNMENT;
+  if (n != 1 && n != batch) return DTA_ERR_SHAPE;
+  *step = n == 1 ? 0 : 1;
+  return DTA_OK;
+}
+
+// Chunk lengths of the dense set: as many chunks as there are CTAs resident at
+// once (kDenseCtasPerSm per SM), at least kDenseChunkMin keys each.
+constexpr int kDenseCtasPerSm = 3;
+constexpr int kDenseChunkMin = 256;
+constexpr int kSparseChunk = 256;
+
+int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
+  if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
+  memset(p, 0, sizeof(*p));
+  const dta_cache_desc& c = a->cache;
+  int st = check_cache(c, &p->log_block, p->side);
+  if (st != DTA_OK) return st;
+  if (a->n_heads <= 0 || a->n_heads % c.n_kv_heads != 0 || a->n_heads / c.n_kv_heads > 8) return DTA_ERR_SHAPE;
+  if (a->n_keys < 0 || a->n_keys > c.capacity) return DTA_ERR_SHAPE;
+  if (a->window < 0 || a->sink < 0) return DTA_ERR_INVALID_ARG;
+  if ((st = check_list(a->n_keys_dev, a->n_lengths, c.batch, &p->len_step)) != DTA_OK) return st;
+  p->B = c.batch; p->H = a->n_heads; p->Hkv = c.n_kv_heads; p->G = a->n_heads / c.n_kv_heads;
+  p->n_keys = a->n_keys;
+  p->n_keys_dev = a->n_keys_dev;
+  p->scale_log2 = a->scaling * 1.4426950408889634f;
+  // sink and window beyond the cache mean the whole cache
+  p->window = a->window < a->n_keys ? a->window : a->n_keys;
+  p->sink = a->sink < a->n_keys ? a->sink : a->n_keys;
+  const long long units = (long long)c.batch * c.n_kv_heads, n = a->n_keys;
+  long long chunk = kDenseChunkMin;
+  if (sms > 0) {
+    const long long want = (units * n + (long long)sms * kDenseCtasPerSm - 1) / ((long long)sms * kDenseCtasPerSm);
+    if (want > chunk) chunk = (want + 63) / 64 * 64;
+  }
+  p->set[0].chunk = (int)chunk;
+  p->set[0].n_launched = (int)((n + chunk - 1) / chunk);
+  p->set[1].chunk = kSparseChunk;
+  p->set[1].n_sink_chunks = (p->sink + kSparseChunk - 1) / kSparseChunk;
+  p->set[1].n_launched = p->set[1].n_sink_chunks + (p->window + kSparseChunk - 1) / kSparseChunk;
+  for (dta::CacheDecodeSet& S : p->set)
+    if (S.n_launched < 1) S.n_launched = 1;  // no keys: one empty partial
+  return DTA_OK;
+}
+
+size_t set_bytes(const dta_cache_decode_args* a, const dta::CacheDecodeSet& S) {
+  return align_up((size_t)a->cache.batch * a->n_heads * S.n_launched * (4 + a->cache.head_dim) * 4, 256);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dta_cache_write(const dta_cache_write_args* a, void* stream) {
+  if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
+  dta::CacheWriteParams p;
+  memset(&p, 0, sizeof(p));
+  const dta_cache_desc& c = a->cache;
+  int st = check_cache(c, &p.log_block, p.side);
+  if (st != DTA_OK) return st;
+  if (!type_ok(a->src_type)) return DTA_ERR_INVALID_ARG;
+  if (a->n_new < 0 || a->n_new > c.capacity) return DTA_ERR_SHAPE;
+  if (!a->pos_dev && (a->pos < 0 || a->pos > c.capacity - a->n_new)) return DTA_ERR_SHAPE;
+  if ((st = check_list(a->pos_dev, a->n_pos, c.batch, &p.pos_step)) != DTA_OK) return st;
+  if ((st = check_list(a->lengths, a->n_lengths, c.batch, &p.len_step)) != DTA_OK) return st;
+  if (a->error_word && !aligned(a->error_word, 4)) return DTA_ERR_ALIGNMENT;
+  if (a->n_new == 0) return DTA_OK;
+  if (!a->k_new || !a->v_new) return DTA_ERR_INVALID_ARG;
+  if (!aligned(a->k_new, 16) || !aligned(a->v_new, 16)) return DTA_ERR_ALIGNMENT;
+  const int es = a->src_type == DTA_CACHE_FP32 ? 4 : 2;
+  const int64_t str[2][3] = {{a->k_new_stride_b, a->k_new_stride_h, a->k_new_stride_s},
+                             {a->v_new_stride_b, a->v_new_stride_h, a->v_new_stride_s}};
+  for (int i = 0; i < 2; ++i) {
+    for (int64_t s : str[i])
+      if (!stride16(s, es)) return DTA_ERR_STRIDE;
+    p.src[i] = i ? a->v_new : a->k_new;
+    p.src_sb[i] = str[i][0]; p.src_sh[i] = str[i][1]; p.src_ss[i] = str[i][2];
+  }
+  int sms = 0;
+  if ((st = dta::check_device(&sms)) != DTA_OK) return st;
+  p.Hkv = c.n_kv_heads; p.n_new = a->n_new; p.capacity = c.capacity;
+  p.pos = a->pos; p.pos_dev = a->pos_dev; p.lengths = a->lengths; p.error_word = a->error_word;
+  const cudaError_t e = dta::launch_cache_write(p, c.batch, c.head_dim, c.format, a->src_type,
+                                                reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? (int)DTA_OK : dta::fail_cuda(e);
+}
+
+int dta_cache_read(const dta_cache_read_args* a, void* stream) {
+  if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
+  dta::CacheReadParams p;
+  memset(&p, 0, sizeof(p));
+  const dta_cache_desc& c = a->cache;
+  int st = check_cache(c, &p.log_block, p.side);
+  if (st != DTA_OK) return st;
+  if (!type_ok(a->dst_type)) return DTA_ERR_INVALID_ARG;
+  if (a->start < 0 || a->n_keys < 0 || a->start > c.capacity || a->n_keys > c.capacity - a->start) return DTA_ERR_SHAPE;
+  if ((st = check_list(a->lengths, a->n_lengths, c.batch, &p.len_step)) != DTA_OK) return st;
+  if (a->n_keys == 0) return DTA_OK;
+  if (!a->out_k || !a->out_v) return DTA_ERR_INVALID_ARG;
+  if (!aligned(a->out_k, 16) || !aligned(a->out_v, 16)) return DTA_ERR_ALIGNMENT;
+  int sms = 0;
+  if ((st = dta::check_device(&sms)) != DTA_OK) return st;
+  p.dst[0] = a->out_k; p.dst[1] = a->out_v;
+  p.Hkv = c.n_kv_heads; p.n = a->n_keys; p.start = a->start; p.lengths = a->lengths;
+  const cudaError_t e = dta::launch_cache_read(p, c.batch, c.head_dim, c.format, a->dst_type,
+                                               reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? (int)DTA_OK : dta::fail_cuda(e);
+}
+
+// Both key sets' partials, whichever outputs the call asks for, at the shortest
+// dense chunk (an upper bound for the chunk dta_cache_decode picks).
+size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
+  dta::CacheDecodeParams p;
+  if (decode_setup(a, &p, 0) != DTA_OK) return 0;
+  return set_bytes(a, p.set[0]) + set_bytes(a, p.set[1]);
+}
+
+int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
+  dta::CacheDecodeParams p;
+  int st = decode_setup(a, &p, 0);
+  if (st != DTA_OK) return st;
+  if (!a->q || (!a->dense_out && !a->sparse_out)) return DTA_ERR_INVALID_ARG;
+  if (!aligned(a->q, 16) || !aligned(a->dense_out, 16) || !aligned(a->sparse_out, 16)) return DTA_ERR_ALIGNMENT;
+  if (!stride16(a->q_stride_b, 2) || !stride16(a->q_stride_h, 2)) return DTA_ERR_STRIDE;
+  const size_t need = dta_cache_decode_workspace_size(a);
+  if (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)) return DTA_ERR_WORKSPACE;
+  int sms = 0;
+  if ((st = dta::check_device(&sms)) != DTA_OK) return st;
+  if ((st = decode_setup(a, &p, sms)) != DTA_OK) return st;  // chunking for this device
+  p.q = reinterpret_cast<const __nv_bfloat16*>(a->q);
+  p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
+  p.set[0].partials = reinterpret_cast<float*>(a->workspace);
+  p.set[1].partials = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + set_bytes(a, p.set[0]));
+  p.out[0] = reinterpret_cast<__nv_bfloat16*>(a->dense_out);
+  p.out[1] = reinterpret_cast<__nv_bfloat16*>(a->sparse_out);
+  const cudaError_t e = dta::launch_cache_decode(p, a->cache.head_dim, a->cache.format, reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? (int)DTA_OK : dta::fail_cuda(e);
+}
+
+}  // extern "C"

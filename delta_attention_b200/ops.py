@@ -15,13 +15,16 @@ caller synchronises anyway) and raises ``DtaError(DTA_ERR_KERNEL_TIMEOUT)``.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import ABI_VERSION, KERNEL_CODES, BackwardArgs, DecodeArgs, DtaError, PrefillArgs, RowsArgs, lib
+from ._lib import (ABI_VERSION, KERNEL_CODES, BackwardArgs, CacheDecodeArgs, CacheReadArgs, CacheWriteArgs,
+                   DecodeArgs, DtaError, PrefillArgs, RowsArgs, lib)
 from ._lib import check as _check_status
+from .kv_cache import QuantizedKV
 
 DTA_ERR_KERNEL_TIMEOUT = 10
 
@@ -428,6 +431,166 @@ def backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
     if check:
         check_errors(q.device)
     return dq, dk, dv
+
+
+# ----------------------------------------------------------------------
+# 8-bit KV cache
+# ----------------------------------------------------------------------
+_CACHE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _on_cache_device(op):
+    """Run an op with its cache's device current: its launches, its stream and
+    its workspace then belong to that device."""
+
+    @functools.wraps(op)
+    def call(*args, **kw):
+        cache = next((x for x in args if isinstance(x, QuantizedKV)), None) or kw.get("cache")
+        if cache is None:
+            raise TypeError(f"{op.__name__} needs a QuantizedKV cache")
+        if cache.device.type != "cuda":
+            raise ValueError("delta_attention_b200 ops take CUDA tensors (there is no CPU path)")
+        if cache.device.index == torch.cuda.current_device():
+            return op(*args, **kw)
+        with torch.cuda.device(cache.device):
+            return op(*args, **kw)
+
+    return call
+
+
+def _device_list(t: torch.Tensor, what: str, cache: QuantizedKV) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.device != cache.device or t.numel() not in (1, cache.batch) or \
+            not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of 1 or {cache.batch} elements on {cache.device}")
+    return t
+
+
+def _cache_source(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [b, h, s, d] if a kernel can read it in place (d contiguous, base
+    and strides multiples of 16 bytes), else an aligned copy."""
+    size, st = t.element_size(), t.stride()
+    if st[3] != 1 or t.data_ptr() % 16 or any(
+            n > 1 and (s <= 0 or s * size % 16) for n, s in zip(t.shape, st[:3])):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+@_on_cache_device
+def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, lengths: Optional[torch.Tensor] = None,
+                check: bool = False) -> None:
+    """Write ``k``, ``v`` [b, Hkv, s, d] (bf16, fp16 or fp32, post-RoPE) into an
+    8-bit cache at positions ``[pos, pos + s)`` of every sequence.
+
+    ``pos`` is an int, or a device int32 tensor of 1 or b elements that the
+    kernel reads (a CUDA graph can then replay the call while the cache
+    grows).  ``lengths`` (device int32, 1 or b elements): only the first
+    ``lengths[i]`` rows of sequence i are written (a padded batch).  Rows
+    before ``pos`` keep their values (a block's scale only rises while it
+    holds earlier rows); rows behind the written ones are no longer live.
+    A device position or length outside the cache writes nothing of that
+    sequence and is recorded in the error word (:func:`check_errors`;
+    ``check=True`` does that right after the launch)."""
+    if k.shape != v.shape or k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (
+            cache.batch, cache.n_kv_heads, cache.head_dim):
+        raise ValueError(f"k and v must be [{cache.batch}, {cache.n_kv_heads}, s, {cache.head_dim}], got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
+        raise ValueError(f"k and v must both be bf16, fp16 or fp32, got {k.dtype} and {v.dtype}")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError(f"k and v must be on the cache's device {cache.device}")
+    s = k.shape[2]
+    if s == 0:
+        return
+    k, v = _cache_source(k), _cache_source(v)
+    a = CacheWriteArgs.from_buffer_copy(cache._write_args)
+    a.n_new, a.src_type = s, _CACHE_TYPES[k.dtype]
+    if isinstance(pos, torch.Tensor):
+        a.pos_dev, a.n_pos = _device_list(pos, "pos", cache).data_ptr(), pos.numel()
+    else:
+        a.pos = int(pos)
+        if not 0 <= a.pos <= cache.capacity - s:
+            raise ValueError(f"positions [{pos}, {pos + s}) are outside the cache of {cache.capacity}")
+    if lengths is not None:
+        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache).data_ptr(), lengths.numel()
+    a.k_new, (a.k_new_stride_b, a.k_new_stride_h, a.k_new_stride_s) = k.data_ptr(), _strides(k)
+    a.v_new, (a.v_new_stride_b, a.v_new_stride_h, a.v_new_stride_s) = v.data_ptr(), _strides(v)
+    a.error_word = error_word(cache.device).data_ptr()
+    _check_status(lib().dta_cache_write(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_write")
+    if check:
+        check_errors(cache.device)
+
+
+@_on_cache_device
+def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int = 0,
+               lengths: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of positions ``[start, start + n_keys)`` (default: to the
+    capacity) as two contiguous [b, Hkv, n_keys, d] tensors of ``dtype`` (bf16,
+    fp16 or fp32), each value rounded once.  ``lengths`` (device int32, 1 or b
+    elements) are the live key counts: rows at or behind them come back as
+    zeros.  ``out`` takes the result instead of new tensors."""
+    n = cache.capacity - start if n_keys is None else int(n_keys)
+    if start < 0 or n < 0 or start + n > cache.capacity:
+        raise ValueError(f"positions [{start}, {start + n}) are outside the cache of {cache.capacity}")
+    if dtype not in _CACHE_TYPES:
+        raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+    shape = (cache.batch, cache.n_kv_heads, n, cache.head_dim)
+    if out is None:
+        out = (torch.empty(shape, dtype=dtype, device=cache.device),
+               torch.empty(shape, dtype=dtype, device=cache.device))
+    else:
+        for t in out:
+            if tuple(t.shape) != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous():
+                raise ValueError(f"out must be two contiguous {shape} {dtype} tensors on {cache.device}")
+    if n == 0:
+        return out
+    a = CacheReadArgs.from_buffer_copy(cache._read_args)
+    a.start, a.n_keys, a.dst_type = int(start), n, _CACHE_TYPES[dtype]
+    a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
+    if lengths is not None:
+        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache).data_ptr(), lengths.numel()
+    _check_status(lib().dta_cache_read(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_read")
+    return out
+
+
+@_on_cache_device
+def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int, scaling: Optional[float] = None,
+                 want_dense: bool = True, want_sparse: bool = True, n_keys: Optional[int] = None,
+                 n_keys_dev: Optional[torch.Tensor] = None,
+                 ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """:func:`decode` over an 8-bit cache: one row per (batch, head), q [b, H, 1, d]
+    (computation from bf16 queries).  Returns ``(dense, sparse)``, each
+    [b, 1, H, d] bf16 or None.  ``n_keys`` live keys (default: the capacity);
+    ``n_keys_dev`` (device int32, 1 or b elements) gives the live counts on the
+    device instead, at most ``n_keys``, which then sizes the launch.  A
+    sequence without keys gets zeros."""
+    b, H, one, d = q.shape
+    if one != 1:
+        raise ValueError("cache_decode takes one query row per (batch, head)")
+    if b != cache.batch or d != cache.head_dim:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of batch {cache.batch}, head_dim {cache.head_dim}")
+    if q.device != cache.device:
+        raise ValueError(f"q must be on the cache's device {cache.device}")
+    if not (want_dense or want_sparse):
+        raise ValueError("neither row is wanted")
+    n = cache.capacity if n_keys is None else int(n_keys)
+    if not 0 <= n <= cache.capacity:
+        raise ValueError(f"n_keys {n} is outside the cache of {cache.capacity}")
+    q = _cache_source(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
+    dense = torch.empty(b, 1, H, d, dtype=torch.bfloat16, device=q.device) if want_dense else None
+    sparse = torch.empty(b, 1, H, d, dtype=torch.bfloat16, device=q.device) if want_sparse else None
+    a = CacheDecodeArgs.from_buffer_copy(cache._decode_args)
+    a.n_heads, a.n_keys, a.window, a.sink = H, n, int(window), int(sink)
+    a.scaling = d ** -0.5 if scaling is None else float(scaling)
+    a.q = q.data_ptr()
+    a.q_stride_b, a.q_stride_h = _strides(q)[:2]
+    a.dense_out, a.sparse_out = _ptr(dense), _ptr(sparse)
+    if n_keys_dev is not None:
+        a.n_keys_dev, a.n_lengths = _device_list(n_keys_dev, "n_keys_dev", cache).data_ptr(), n_keys_dev.numel()
+    ws = _decode_workspace(lib().dta_cache_decode_workspace_size(ctypes.byref(a)), cache.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _check_status(lib().dta_cache_decode(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_decode")
+    return dense, sparse
 
 
 def check_workspace(workspace: torch.Tensor) -> int:

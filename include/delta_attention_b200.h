@@ -261,6 +261,103 @@ typedef struct dta_backward_args {
 DTA_API size_t dta_backward_workspace_size(const dta_backward_args* args);
 DTA_API int dta_backward(const dta_backward_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit KV cache.  No counterpart in the reference (it is an addition of this
+ * library).  The keys and values of one layer are held as 8-bit codes
+ * [batch, n_kv_heads, capacity, head_dim] (strides in bytes: multiples of 16,
+ * head_dim contiguous) with one scale byte u for each block of `block` tokens and
+ * head, [batch, n_kv_heads, ceil(capacity / block)] (last stride 1): a code c
+ * stands for c * 2^(u - 127) (E8M0).  A block's u is the smallest >= 1 with
+ * amax <= qmax * 2^(u - 127), amax the largest finite magnitude written to it.
+ * e4m3: a non-finite value is held as NaN.  int8: codes lie in [-127, 127], and a
+ * block given a non-finite value has u = 255 and reads as NaN. */
+typedef enum dta_cache_format {
+  DTA_CACHE_E4M3 = 0, /* qmax 448 */
+  DTA_CACHE_INT8 = 1  /* qmax 127 */
+} dta_cache_format;
+
+/* Element types of the 16- and 32-bit side. */
+typedef enum dta_cache_type { DTA_CACHE_BF16 = 0, DTA_CACHE_FP16 = 1, DTA_CACHE_FP32 = 2 } dta_cache_type;
+
+typedef struct dta_cache_desc {
+  int32_t batch, n_kv_heads, capacity, head_dim;
+  int32_t block;            /* tokens per scale: 16, 32, 64 or 128 */
+  int32_t format;           /* dta_cache_format */
+  void* k;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  void* v;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  uint8_t* k_scale;
+  int64_t k_scale_stride_b, k_scale_stride_h;
+  uint8_t* v_scale;
+  int64_t v_scale_stride_b, v_scale_stride_h;
+} dta_cache_desc;
+
+/* Write n_new rows of K and V per sequence at positions [pos, pos + n_new).
+ * k_new, v_new: [batch, n_kv_heads, n_new, head_dim] of src_type (strides in
+ * elements; head_dim contiguous, strides and base 16-byte aligned).
+ * Rows that the touched blocks hold before pos are kept: such a block's scale never
+ * falls, and where it rises their codes are rounded to the new one.  Rows behind the
+ * written ones are no longer live (in a touched block their scale may have changed;
+ * other blocks are left as they are). */
+typedef struct dta_cache_write_args {
+  int32_t abi_version;
+  int32_t n_new;            /* 0 writes nothing */
+  int32_t src_type;         /* dta_cache_type */
+  int32_t pos;              /* first position, 0 <= pos, pos + n_new <= capacity (pos_dev NULL) */
+  dta_cache_desc cache;
+  const void* k_new;
+  int64_t k_new_stride_b, k_new_stride_h, k_new_stride_s;
+  const void* v_new;
+  int64_t v_new_stride_b, v_new_stride_h, v_new_stride_s;
+  const int32_t* pos_dev;   /* optional device int32 [n_pos]: first position, read by the kernel */
+  int32_t n_pos;            /* 1 (the same for every sequence) or batch */
+  int32_t n_lengths;        /* 1 or batch */
+  const int32_t* lengths;   /* optional device int32 [n_lengths]: rows of each sequence that are written,
+                               0 <= length <= n_new */
+  int32_t* error_word;      /* as in dta_prefill_args: code 105 for a device position or length outside the
+                               cache, whose sequence is then not written */
+} dta_cache_write_args;
+DTA_API int dta_cache_write(const dta_cache_write_args* args, void* stream);
+
+/* Read rows [start, start + n_keys) back: out_k, out_v [batch, n_kv_heads, n_keys,
+ * head_dim] of dst_type, contiguous, 16-byte aligned. */
+typedef struct dta_cache_read_args {
+  int32_t abi_version;
+  int32_t start, n_keys;    /* n_keys 0 reads nothing */
+  int32_t dst_type;         /* dta_cache_type */
+  dta_cache_desc cache;
+  void* out_k;
+  void* out_v;
+  const int32_t* lengths;   /* optional device int32 [n_lengths]: live keys of each sequence; rows at or
+                               behind that count are written as zeros */
+  int32_t n_lengths;        /* 1 or batch */
+} dta_cache_read_args;
+DTA_API int dta_cache_read(const dta_cache_read_args* args, void* stream);
+
+/* dta_decode over an 8-bit cache: the dense and / or sparse row of every (batch,
+ * head), same key sets.  q: [batch, n_heads, 1, head_dim] bf16; outputs
+ * [batch, 1, n_heads, head_dim] bf16.  A sequence without keys gets zeros. */
+typedef struct dta_cache_decode_args {
+  int32_t abi_version;
+  int32_t n_heads;
+  int32_t n_keys;           /* live keys of every sequence; with n_keys_dev an upper bound of them */
+  int32_t window, sink;
+  float scaling;
+  dta_cache_desc cache;
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  void* dense_out;
+  void* sparse_out;
+  const int32_t* n_keys_dev; /* optional device int32 [n_lengths]: live keys, read by the kernels and clamped to
+                                [0, n_keys] */
+  int32_t n_lengths;         /* 1 or batch */
+  void* workspace;           /* nothing in it needs to start at zero */
+  size_t workspace_bytes;
+} dta_cache_decode_args;
+DTA_API size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* args);
+DTA_API int dta_cache_decode(const dta_cache_decode_args* args, void* stream);
+
 /* Host-side helpers. */
 DTA_API int dta_abi_version(void);
 DTA_API const char* dta_status_string(int status);
