@@ -52,7 +52,10 @@ int check_list(const int32_t* list, int n, int batch, int* step) {
 
 // Chunk lengths of the dense set: as many chunks as there are CTAs resident at
 // once (kDenseCtasPerSm per SM), at least kDenseChunkMin keys each.
-constexpr int kDenseCtasPerSm = 3;
+#ifndef DTA_CD_CTAS
+#define DTA_CD_CTAS 2
+#endif
+constexpr int kDenseCtasPerSm = DTA_CD_CTAS;
 constexpr int kDenseChunkMin = 256;
 constexpr int kSparseChunk = 256;
 

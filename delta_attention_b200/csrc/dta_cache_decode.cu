@@ -25,8 +25,19 @@
 
 namespace dta {
 
-constexpr int CD_WARPS = 4;
+#ifndef DTA_CD_KEYS
+#define DTA_CD_KEYS 32
+#endif
+#ifndef DTA_CD_STAGES
+#define DTA_CD_STAGES 3
+#endif
+#ifndef DTA_CD_WARPS
+#define DTA_CD_WARPS 4
+#endif
+constexpr int CD_WARPS = DTA_CD_WARPS;
 constexpr int CD_THREADS = CD_WARPS * 32;
+constexpr int CD_KEYS = DTA_CD_KEYS;      // keys per step of a warp
+constexpr int CD_STAGES = DTA_CD_STAGES;  // steps in flight per warp
 constexpr float CD_SHIFT = 14.f;  // log2 of the factor that the fp16 weights carry
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -48,14 +59,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-
 __device__ __forceinline__ int cd_live(const CacheDecodeParams& p, int b) {
   if (!p.n_keys_dev) return p.n_keys;
   return min(max(p.n_keys_dev[b * p.len_step], 0), p.n_keys);
@@ -82,21 +85,40 @@ __device__ __forceinline__ void cd_range(const CacheDecodeParams& p, const Cache
   k1 = max(k1, k0);
 }
 
-// One group of 16 keys as a warp holds it: K for lane (g, t) = (lane / 4, lane % 4):
-// keys g and 8 + g, 16-byte pieces t and t + 4 of the row; V: keys 2t, 2t+1, 2t+8,
-// 2t+9, bytes [HD/8 * g, HD/8 * (g + 1)).
+// Shared-memory ring of one warp: CD_STAGES stages of CD_KEYS keys, each K rows
+// then V rows of HD bytes.  The 16-byte pieces of row r are permuted by r, so
+// that the fragment reads below are free of bank conflicts (HD = 128; at 64 the
+// reads of V take two passes).
 template <int HD>
-struct Group {
-  static constexpr int KP = HD / 64;       // 16-byte pieces per lane and key of K
-  static constexpr int VW = HD / 32;       // words per lane and key of V
-  uint32_t k[2][KP][4];
-  uint32_t v[4][VW];
-  int ku, vu;                              // scale bytes
-};
+__device__ __forceinline__ int cd_swizzle(int row, int piece) {
+  return HD == 128 ? piece ^ (row & 7) : piece ^ (row & 2);
+}
+template <int HD>
+__host__ __device__ constexpr int cd_smem() {
+  return CD_WARPS * CD_STAGES * 2 * CD_KEYS * HD;
+}
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&w)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+}
+__device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
 
+// Partial kernel: CD_WARPS warps, each with a ring and a state of its own; warp w
+// takes the chunk's keys in steps of CD_KEYS, every CD_WARPS-th step.  With
+// (g, t) = (lane / 4, lane % 4) a step is, for each group of 16 keys,
+//   S^T (16 keys x 8 heads) = K Q^T   m16n8k16, A rows g and 8 + g = those keys;
+//                                     lane t holds pieces KP t + c of a row, and its
+//                                     word i of piece c feeds step (c, i)
+//   O^T (dims x 8 heads) += V^T P^T   lane (g, t) holds bytes [HD/8 g, HD/8 (g + 1)) of
+//                                     keys 2t, 2t+1, 2t+8, 2t+9: rows g and 8 + g of
+//                                     tile j are dims HD/8 g + 2j and + 1
+// so that codes go from shared memory into fragments without any exchange; only
+// the weights are transposed (movmatrix).
 template <int HD, int FMT>
 __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_constant__ CacheDecodeParams p, int which) {
-  constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16;
+  constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16, NG = CD_KEYS / CACHE_GROUP;
+  extern __shared__ __align__(128) uint8_t cd_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int b = blockIdx.y / p.Hkv, hk = blockIdx.y - b * p.Hkv;
@@ -110,25 +132,57 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
   const uint8_t* vc = p.side[1].codes + (long long)b * p.side[1].sb + (long long)hk * p.side[1].sh;
   const uint8_t* ks = p.side[0].scale + (long long)b * p.side[0].scale_sb + (long long)hk * p.side[0].scale_sh;
   const uint8_t* vs = p.side[1].scale + (long long)b * p.side[1].scale_sb + (long long)hk * p.side[1].scale_sh;
+  const long long kss = p.side[0].ss, vss = p.side[1].ss;
 
-  // Q as the B operand: head g, dims 16 (t + 4c) + 4i + {0, 1} and + {2, 3} for
-  // step (c, i), the dims that word i of a lane's piece c holds
+  // ---- copies: lane -> piece lane % PC of rows lane / PC, + 32 / PC, ... ----
+  constexpr int PC = HD / 16, RL = 32 / PC;  // pieces per row, rows per pass
+  constexpr int STAGE = 2 * CD_KEYS * HD;
+  const uint32_t ring = smem_u32(cd_ring) + warp * CD_STAGES * STAGE;
+  const int cr = lane / PC, cp = lane % PC;
+  const int a0 = (k0 & ~(CACHE_GROUP - 1)) + warp * CD_KEYS;
+  constexpr int STRIDE = CD_WARPS * CD_KEYS;
+  const int steps = k1 > a0 ? (k1 - a0 + STRIDE - 1) / STRIDE : 0;
+  auto issue = [&](int step, int slot) {
+    const int base = a0 + step * STRIDE;
+    const uint32_t dst = ring + slot * STAGE;
+    const bool whole = base >= k0 && base + CD_KEYS <= k1;
+    const uint8_t* ksrc = kc + (long long)(base + cr) * kss + cp * 16;
+    const uint8_t* vsrc = vc + (long long)(base + cr) * vss + cp * 16;
+#pragma unroll
+    for (int i = 0; i < CD_KEYS / RL; ++i) {
+      const int row = cr + i * RL, key = base + row;
+      const bool ok = whole || (key >= k0 && key < k1);
+      const uint32_t off = dst + row * HD + (cd_swizzle<HD>(row, cp) << 4);
+      // rows outside the chunk are filled with zeros (a masked value must not be NaN: 0 * NaN)
+      cp_async_16(off, ok ? ksrc + i * RL * kss : kc + (long long)k0 * kss, ok ? 16u : 0u);
+      cp_async_16(off + CD_KEYS * HD, ok ? vsrc + i * RL * vss : vc + (long long)k0 * vss, ok ? 16u : 0u);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < CD_STAGES - 1; ++s) {
+    if (s < steps) issue(s, s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // ---- Q as the B operand: head g, dims 16 (KP t + c) + 4 i + {0, 1} and + {2, 3} for step (c, i) ----
   uint32_t qb[KP][4][2];
   float my_scale;
   {
     const bool hv = g < G;
     const __nv_bfloat16* qp = p.q + (long long)b * p.q_sb + (long long)(hk * G + (hv ? g : 0)) * p.q_sh;
-    uint4 raw[KP][2];
+    uint32_t w[KP][8];
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < KP; ++c)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        raw[c][i] = hv ? reinterpret_cast<const uint4*>(qp + 16 * (t + 4 * c))[i] : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max((w[e] << 16) & 0x7fffffffu, w[e] & 0x7fff0000u));
+        const uint4 x = hv ? reinterpret_cast<const uint4*>(qp + 16 * (KP * t + c))[i] : make_uint4(0, 0, 0, 0);
+        w[c][4 * i] = x.x; w[c][4 * i + 1] = x.y; w[c][4 * i + 2] = x.z; w[c][4 * i + 3] = x.w;
       }
+#pragma unroll
+    for (int c = 0; c < KP; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, max((w[c][e] << 16) & 0x7fffffffu, w[c][e] & 0x7fff0000u));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // bring the largest magnitude to [2^14, 2^15); a row with a non-finite element is NaN throughout
@@ -139,13 +193,9 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
 #pragma unroll
     for (int c = 0; c < KP; ++c)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2)
-          qb[c][2 * i + (e2 >> 1)][e2 & 1] =
-              pack_f16x2(__uint_as_float(w[e2] << 16) * f, __uint_as_float(w[e2] & 0xffff0000u) * f);
-      }
+      for (int x = 0; x < 8; ++x)
+        qb[c][x >> 1][x & 1] =
+            pack_f16x2(__uint_as_float(w[c][x] << 16) * f, __uint_as_float(w[c][x] & 0xffff0000u) * f);
   }
   // score factors of this lane's columns, heads 2t and 2t + 1
   float sl[2];
@@ -157,120 +207,164 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-  auto load = [&](int base, Group<HD>& x) {
-    const bool whole = base >= k0 && base + CACHE_GROUP <= k1;
+  // fragment read offsets within a stage (the pieces' permutation depends on the lane alone)
+  uint32_t ka[KP], va[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int key = base + 8 * e + g;
-      const bool ok = whole || (key >= k0 && key < k1);
+  for (int c = 0; c < KP; ++c) ka[c] = g * HD + (cd_swizzle<HD>(g, KP * t + c) << 4);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    va[e] = CD_KEYS * HD + (2 * t + e) * HD + (cd_swizzle<HD>(2 * t + e, HD == 128 ? g : g >> 1) << 4) +
+            (HD == 128 ? 0 : 8 * (g & 1));
+
+  int slot = 0;
+  for (int step = 0; step < steps; ++step) {
+    const int base = a0 + step * STRIDE;
+    const uint32_t st = ring + slot * STAGE;
+    // this step's scale bytes (a group behind the chunk takes the last key's block)
+    int ku[NG], vu[NG];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int blk = min(base + q * CACHE_GROUP, k1 - 1) >> p.log_block;
+      ku[q] = ks[blk];
+      vu[q] = vs[blk];
+    }
+    {
+      const int next = step + CD_STAGES - 1;
+      int ns = slot + CD_STAGES - 1;
+      if (ns >= CD_STAGES) ns -= CD_STAGES;
+      if (next < steps) issue(next, ns);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(CD_STAGES - 1) : "memory");
+    __syncwarp();
+
+    // ---- scores ----
+    float s[NG][4];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KP; ++c) {
-        const uint4 w = ok ? ld_stream16(kc + (long long)key * p.side[0].ss + 16 * (t + 4 * c)) : make_uint4(0, 0, 0, 0);
-        x.k[e][c][0] = w.x; x.k[e][c][1] = w.y; x.k[e][c][2] = w.z; x.k[e][c][3] = w.w;
+        uint32_t w0[4], w1[4];
+        lds128(st + ka[c] + (q * CACHE_GROUP) * HD, w0);
+        lds128(st + ka[c] + (q * CACHE_GROUP + 8) * HD, w1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = cache_bias<FMT>(w0[i]), y = cache_bias<FMT>(w1[i]);
+          mma_f16(s[q], cache_half2<FMT, 0>(x), cache_half2<FMT, 0>(y), cache_half2<FMT, 1>(x), cache_half2<FMT, 1>(y),
+                  qb[c][i][0], qb[c][i][1]);
+        }
       }
     }
+    // ---- weights ----
+    float ve[NG];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int key = base + 8 * (e >> 1) + 2 * t + (e & 1);
-      const bool ok = whole || (key >= k0 && key < k1);  // (a masked value must not be NaN: 0 * NaN)
-      const uint8_t* src = vc + (long long)key * p.side[1].ss + 4 * VW * g;
-      if constexpr (VW == 4) {
-        const uint4 w = ok ? ld_stream16(src) : make_uint4(0, 0, 0, 0);
-        x.v[e][0] = w.x; x.v[e][1] = w.y; x.v[e][2] = w.z; x.v[e][3] = w.w;
-      } else {
-        const uint2 w = ok ? *reinterpret_cast<const uint2*>(src) : make_uint2(0, 0);
-        x.v[e][0] = w.x; x.v[e][1] = w.y;
-      }
+    for (int q = 0; q < NG; ++q) {
+      const float kf = cache_scale(ku[q]);
+      ve[q] = vu[q] == 255 ? __uint_as_float(0x7fc00000u) : (float)(vu[q] - 127);
+      s[q][0] *= sl[0] * kf;
+      s[q][1] *= sl[1] * kf;
+      s[q][2] *= sl[0] * kf;
+      s[q][3] *= sl[1] * kf;
     }
-    const int blk = base >> p.log_block;
-    x.ku = ks[blk];
-    x.vu = vs[blk];
-  };
-
-  auto step = [&](int base, const Group<HD>& x) {
-    // S^T (keys x heads) = K Q^T
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (base < k0 || base + CD_KEYS > k1) {
 #pragma unroll
-    for (int c = 0; c < KP; ++c)
+      for (int q = 0; q < NG; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w0 = cache_bias<FMT>(x.k[0][c][i]), w1 = cache_bias<FMT>(x.k[1][c][i]);
-        mma_f16(s, cache_half2<FMT, 0>(w0), cache_half2<FMT, 0>(w1), cache_half2<FMT, 1>(w0), cache_half2<FMT, 1>(w1),
-                qb[c][i][0], qb[c][i][1]);
-      }
-    const float kf = cache_scale(x.ku);
-    const float ve = x.vu == 255 ? __uint_as_float(0x7fc00000u) : (float)(x.vu - 127);
-    const int key = base + g;
-    const bool ok0 = key >= k0 && key < k1, ok1 = key + 8 >= k0 && key + 8 < k1;
-    float pw[4];
+        for (int e = 0; e < 2; ++e) {
+          const int key = base + q * CACHE_GROUP + 8 * e + g;
+          if (key < k0 || key >= k1) s[q][2 * e] = s[q][2 * e + 1] = -INFINITY;
+        }
+    }
+    float mx[2], rx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = sl[h] * kf;
-      const float s0 = ok0 ? s[h] * f : -INFINITY, s1 = ok1 ? s[2 + h] * f : -INFINITY;
-      float mx = fmaxf(s0, s1);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float mn = fmaxf(m[h], mx), rn = fmaxf(r[h], mx + ve);
-      const float mu = mn == -INFINITY ? 0.f : mn, ru = rn == -INFINITY ? 0.f : rn;
-      const float am = fast_exp2(m[h] - mu), ar = fast_exp2(r[h] - ru);
-      m[h] = mn;
-      r[h] = rn;
-      l[h] = l[h] * am + fast_exp2(s0 - mu) + fast_exp2(s1 - mu);
-      const float off = ve - ru + CD_SHIFT;
-      pw[h] = fast_exp2(s0 + off);
-      pw[2 + h] = fast_exp2(s1 + off);
+      mx[h] = rx[h] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        o[j][h] *= ar;
-        o[j][2 + h] *= ar;
+      for (int q = 0; q < NG; ++q) {
+        const float x = fmaxf(s[q][h], s[q][2 + h]);
+        mx[h] = fmaxf(mx[h], x);
+        rx[h] = fmaxf(rx[h], x + ve[q]);
+      }
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], d));
+        rx[h] = fmaxf(rx[h], __shfl_xor_sync(0xffffffffu, rx[h], d));
       }
     }
-    // P^T as the B operand: keys 2t, 2t+1 (and 8 more), head g
-    const uint32_t b0 = movmatrix_t(pack_f16x2(pw[0], pw[1]));
-    const uint32_t b1 = movmatrix_t(pack_f16x2(pw[2], pw[3]));
-    // O^T (dims x heads) += V^T P^T; rows g and 8 + g of tile j are dims HD/8 g + 2j, + 1
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || rx[0] > r[0] || rx[1] > r[1])) {
 #pragma unroll
-    for (int i = 0; i < VW; ++i) {
-      const uint32_t wa = cache_bias<FMT>(x.v[0][i]), wb = cache_bias<FMT>(x.v[1][i]);
-      const uint32_t wc = cache_bias<FMT>(x.v[2][i]), wd = cache_bias<FMT>(x.v[3][i]);
-      const uint32_t ab = __byte_perm(wa, wb, 0x5140), AB = __byte_perm(wa, wb, 0x7362);
-      const uint32_t cd = __byte_perm(wc, wd, 0x5140), CD = __byte_perm(wc, wd, 0x7362);
-      mma_f16(o[2 * i], cache_half2<FMT, 0>(ab), cache_half2<FMT, 1>(ab), cache_half2<FMT, 0>(cd),
-              cache_half2<FMT, 1>(cd), b0, b1);
-      mma_f16(o[2 * i + 1], cache_half2<FMT, 0>(AB), cache_half2<FMT, 1>(AB), cache_half2<FMT, 0>(CD),
-              cache_half2<FMT, 1>(CD), b0, b1);
+      for (int h = 0; h < 2; ++h) {
+        const float mn = fmaxf(m[h], mx[h]), rn = fmaxf(r[h], rx[h]);
+        const float am = m[h] == mn ? 1.f : fast_exp2(m[h] - mn), ar = r[h] == rn ? 1.f : fast_exp2(r[h] - rn);
+        m[h] = mn;
+        r[h] = rn;
+        l[h] *= am;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          o[j][h] *= ar;
+          o[j][2 + h] *= ar;
+        }
+      }
     }
-  };
-
-  const int first = (k0 & ~(CACHE_GROUP - 1)) + warp * CACHE_GROUP;
-  constexpr int STEP = CD_WARPS * CACHE_GROUP;
-  Group<HD> x;
-  if (first < k1) load(first, x);
-  for (int base = first; base < k1; base += STEP) {
-    Group<HD> nx;
-    if (base + STEP < k1) load(base + STEP, nx);
-    step(base, x);
-    x = nx;
+    const float mu[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float ru[2] = {r[0] == -INFINITY ? 0.f : r[0], r[1] == -INFINITY ? 0.f : r[1]};
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      float pw[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += fast_exp2(s[q][h] - mu[h]) + fast_exp2(s[q][2 + h] - mu[h]);
+        const float off = ve[q] - ru[h] + CD_SHIFT;
+        pw[h] = fast_exp2(s[q][h] + off);
+        pw[2 + h] = fast_exp2(s[q][2 + h] + off);
+      }
+      const uint32_t b0 = movmatrix_t(pack_f16x2(pw[0], pw[1]));
+      const uint32_t b1 = movmatrix_t(pack_f16x2(pw[2], pw[3]));
+      // ---- values ----
+      uint32_t v[4][VW];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t addr = st + va[e & 1] + (q * CACHE_GROUP + 8 * (e >> 1)) * HD;
+        if constexpr (VW == 4) lds128(addr, v[e]);
+        else lds64(addr, v[e]);
+      }
+#pragma unroll
+      for (int i = 0; i < VW; ++i) {
+        const uint32_t wa = cache_bias<FMT>(v[0][i]), wb = cache_bias<FMT>(v[1][i]);
+        const uint32_t wc = cache_bias<FMT>(v[2][i]), wd = cache_bias<FMT>(v[3][i]);
+        const uint32_t ab = __byte_perm(wa, wb, 0x5140), AB = __byte_perm(wa, wb, 0x7362);
+        const uint32_t cd = __byte_perm(wc, wd, 0x5140), CD = __byte_perm(wc, wd, 0x7362);
+        mma_f16(o[2 * i], cache_half2<FMT, 0>(ab), cache_half2<FMT, 1>(ab), cache_half2<FMT, 0>(cd),
+                cache_half2<FMT, 1>(cd), b0, b1);
+        mma_f16(o[2 * i + 1], cache_half2<FMT, 0>(AB), cache_half2<FMT, 1>(AB), cache_half2<FMT, 0>(CD),
+                cache_half2<FMT, 1>(CD), b0, b1);
+      }
+    }
+    __syncwarp();  // the slot may be refilled
+    if (++slot == CD_STAGES) slot = 0;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-  // merge the warps through shared memory
-  __shared__ float red_o[CD_WARPS][8][HD];
-  __shared__ float red_s[CD_WARPS][3][8];
+  // ---- merge the warps through shared memory (their rings are done with) ----
+  __syncthreads();
+  float* red_o = reinterpret_cast<float*>(cd_ring);  // [CD_WARPS][8][HD]
+  float* red_s = red_o + CD_WARPS * 8 * HD;          // [CD_WARPS][3][8]
+  static_assert(cd_smem<HD>() >= (CD_WARPS * 8 * HD + CD_WARPS * 24) * 4, "merge buffers fit in the rings");
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
     if (g == 0) {
-      red_s[warp][0][2 * t + h] = m[h];
-      red_s[warp][1][2 * t + h] = l[h];
-      red_s[warp][2][2 * t + h] = r[h];
+      red_s[warp * 24 + 2 * t + h] = m[h];
+      red_s[warp * 24 + 8 + 2 * t + h] = l[h];
+      red_s[warp * 24 + 16 + 2 * t + h] = r[h];
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      red_o[warp][2 * t + h][HD / 8 * g + 2 * j] = o[j][h];
-      red_o[warp][2 * t + h][HD / 8 * g + 2 * j + 1] = o[j][2 + h];
+      red_o[(warp * 8 + 2 * t + h) * HD + HD / 8 * g + 2 * j] = o[j][h];
+      red_o[(warp * 8 + 2 * t + h) * HD + HD / 8 * g + 2 * j + 1] = o[j][2 + h];
     }
   }
   __syncthreads();
@@ -280,15 +374,15 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     float M = -INFINITY, R = -INFINITY;
 #pragma unroll
     for (int w = 0; w < CD_WARPS; ++w) {
-      M = fmaxf(M, red_s[w][0][h]);
-      R = fmaxf(R, red_s[w][2][h]);
+      M = fmaxf(M, red_s[w * 24 + h]);
+      R = fmaxf(R, red_s[w * 24 + 16 + h]);
     }
     float L = 0.f, O = 0.f;
 #pragma unroll
     for (int w = 0; w < CD_WARPS; ++w) {
-      if (red_s[w][1][h] == 0.f) continue;  // no key of this warp counts
-      L += red_s[w][1][h] * fast_exp2(red_s[w][0][h] - M);
-      O += red_o[w][h][d] * fast_exp2(red_s[w][2][h] - R);
+      if (red_s[w * 24 + 8 + h] == 0.f) continue;  // no key of this warp counts
+      L += red_s[w * 24 + 8 + h] * fast_exp2(red_s[w * 24 + h] - M);
+      O += red_o[(w * 8 + h) * HD + d] * fast_exp2(red_s[w * 24 + 16 + h] - R);
     }
     float* part = part0 + (long long)h * S.n_launched * (4 + HD);
     part[4 + d] = O;
@@ -300,26 +394,66 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
   }
 }
 
-// Merge of a key set's partials: grid (B * H), one thread per head dim.
+// Merge of a key set's partials: grid (B * H, key sets), MG_THREADS / HD threads per
+// head dim.  The threads' columns of the first MG_THREADS / HD * MG_LOADS chunks are on their
+// way while the chunks' weights are formed, so a set of up to that many chunks
+// costs one round trip to L2.  A programmatic dependent launch: its CTAs are
+// resident when the partials' grid ends.
+constexpr int MG_THREADS = 512, MG_LOADS = 8;
+
 template <int HD>
-__global__ void cache_merge_kernel(const __grid_constant__ CacheDecodeParams p) {
-  const int bh = blockIdx.x, d = threadIdx.x;
+__global__ void __launch_bounds__(MG_THREADS) cache_merge_kernel(const __grid_constant__ CacheDecodeParams p) {
+  constexpr int ROWS = MG_THREADS / HD, TILE = ROWS * MG_LOADS;
+  __shared__ float wl[TILE], wo[TILE], hm[TILE], hr[TILE];
+  __shared__ float red[ROWS][HD];
+  const int bh = blockIdx.x, which = p.out[0] ? blockIdx.y : 1;
+  const int d = threadIdx.x % HD, y = threadIdx.x / HD;
+  const CacheDecodeSet& S = p.set[which];
+  const float* base = S.partials + (long long)bh * S.n_launched * (4 + HD);
   grid_dependency_wait();
-  for (int which = 0; which < 2; ++which) {
-    if (!p.out[which]) continue;
-    const CacheDecodeSet& S = p.set[which];
-    const float* base = S.partials + (long long)bh * S.n_launched * (4 + HD);
-    float M = -INFINITY, R = -INFINITY, L = 0.f, O = 0.f;
-    for (int x = 0; x < S.n_launched; ++x) {
-      const float* part = base + (long long)x * (4 + HD);
-      const float m = part[0], l = part[1], r = part[2], o = part[4 + d];
-      if (l == 0.f) continue;
-      const float mn = fmaxf(M, m), rn = fmaxf(R, r);
-      L = L * fast_exp2(M - mn) + l * fast_exp2(m - mn);
-      O = O * fast_exp2(R - rn) + o * fast_exp2(r - rn);
-      M = mn;
-      R = rn;
+  float M = -INFINITY, R = -INFINITY, L = 0.f, O = 0.f;
+  for (int x0 = 0; x0 < S.n_launched; x0 += TILE) {
+    const int n = min(TILE, S.n_launched - x0);
+    const float* tile = base + (long long)x0 * (4 + HD);
+    float ov[MG_LOADS];
+#pragma unroll
+    for (int i = 0; i < MG_LOADS; ++i) {
+      const int x = y + i * ROWS;
+      ov[i] = x < n ? tile[(long long)x * (4 + HD) + 4 + d] : 0.f;
     }
+    float l = 0.f;
+    if (threadIdx.x < TILE) {
+      float4 h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      if ((int)threadIdx.x < n) h = *reinterpret_cast<const float4*>(tile + (long long)threadIdx.x * (4 + HD));
+      l = h.y;
+      hm[threadIdx.x] = h.x;
+      hr[threadIdx.x] = h.z;
+    }
+    __syncthreads();
+    float mt = M, rt = R;
+    for (int x = 0; x < n; ++x) {
+      mt = fmaxf(mt, hm[x]);
+      rt = fmaxf(rt, hr[x]);
+    }
+    if (threadIdx.x < TILE) {  // a chunk without keys has no weight
+      wl[threadIdx.x] = l == 0.f ? 0.f : l * fast_exp2(hm[threadIdx.x] - mt);
+      wo[threadIdx.x] = l == 0.f ? 0.f : fast_exp2(hr[threadIdx.x] - rt);
+    }
+    __syncthreads();
+    if (M != mt) L *= fast_exp2(M - mt);
+    if (R != rt) O *= fast_exp2(R - rt);
+    M = mt;
+    R = rt;
+    for (int x = 0; x < n; ++x) L += wl[x];
+#pragma unroll
+    for (int i = 0; i < MG_LOADS; ++i) O += wo[y + i * ROWS] == 0.f ? 0.f : ov[i] * wo[y + i * ROWS];
+    __syncthreads();
+  }
+  red[y][d] = O;
+  __syncthreads();
+  if (y == 0) {
+#pragma unroll
+    for (int i = 1; i < ROWS; ++i) O += red[i][d];
     const float v = L == 0.f ? 0.f : (O * 0x1p-14f) * exp2f(R - M) / L;
     p.out[which][(long long)bh * HD + d] = __float2bfloat16_rn(v);
   }
@@ -327,13 +461,25 @@ __global__ void cache_merge_kernel(const __grid_constant__ CacheDecodeParams p) 
 
 template <int HD, int FMT>
 static cudaError_t decode_as(const CacheDecodeParams& p, cudaStream_t stream) {
+  constexpr int smem = cd_smem<HD>();
+  auto kernel = cache_decode_kernel<HD, FMT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
   for (int which = 0; which < 2; ++which)
     if (p.out[which])
-      cache_decode_kernel<HD, FMT><<<dim3(p.set[which].n_launched, p.B * p.Hkv), CD_THREADS, 0, stream>>>(p, which);
-  cudaError_t e = cudaGetLastError();
+      kernel<<<dim3(p.set[which].n_launched, p.B * p.Hkv), CD_THREADS, smem, stream>>>(p, which);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cache_merge_kernel<HD><<<p.B * p.H, HD, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.B * p.H, (p.out[0] ? 1 : 0) + (p.out[1] ? 1 : 0));
+  cfg.blockDim = dim3(MG_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache_merge_kernel<HD>, p);
 }
 
 cudaError_t launch_cache_decode(const CacheDecodeParams& p, int head_dim, int format, cudaStream_t stream) {
