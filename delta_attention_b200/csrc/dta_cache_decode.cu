@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "dta_cache.h"
 #include "dta_cache_codes.cuh"
 #include "dta_ptx.cuh"
@@ -142,20 +144,42 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
   const int a0 = (k0 & ~(CACHE_GROUP - 1)) + warp * CD_KEYS;
   constexpr int STRIDE = CD_WARPS * CD_KEYS;
   const int steps = k1 > a0 ? (k1 - a0 + STRIDE - 1) / STRIDE : 0;
+  // shared-memory offsets of this lane's pieces of its first and second row (the
+  // permutation repeats after two passes)
+  const uint32_t c0 = cr * HD + (cd_swizzle<HD>(cr, cp) << 4);
+  const uint32_t c1 = (cr + RL) * HD + (cd_swizzle<HD>(cr + RL, cp) << 4);
+  const bool packed = kss == HD && vss == HD;
   auto issue = [&](int step, int slot) {
     const int base = a0 + step * STRIDE;
     const uint32_t dst = ring + slot * STAGE;
-    const bool whole = base >= k0 && base + CD_KEYS <= k1;
     const uint8_t* ksrc = kc + (long long)(base + cr) * kss + cp * 16;
     const uint8_t* vsrc = vc + (long long)(base + cr) * vss + cp * 16;
+    if (base >= k0 && base + CD_KEYS <= k1) {
+      if (packed) {  // rows follow one another: every offset is a constant
 #pragma unroll
-    for (int i = 0; i < CD_KEYS / RL; ++i) {
-      const int row = cr + i * RL, key = base + row;
-      const bool ok = whole || (key >= k0 && key < k1);
-      const uint32_t off = dst + row * HD + (cd_swizzle<HD>(row, cp) << 4);
+        for (int i = 0; i < CD_KEYS / RL; ++i)
+          cp_async_16(dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD, ksrc + i * RL * HD, 16u);
+#pragma unroll
+        for (int i = 0; i < CD_KEYS / RL; ++i)
+          cp_async_16(dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD + CD_KEYS * HD, vsrc + i * RL * HD, 16u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CD_KEYS / RL; ++i) {
+          const uint32_t off = dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD;
+          cp_async_16(off, ksrc + i * RL * kss, 16u);
+          cp_async_16(off + CD_KEYS * HD, vsrc + i * RL * vss, 16u);
+        }
+      }
+    } else {
       // rows outside the chunk are filled with zeros (a masked value must not be NaN: 0 * NaN)
-      cp_async_16(off, ok ? ksrc + i * RL * kss : kc + (long long)k0 * kss, ok ? 16u : 0u);
-      cp_async_16(off + CD_KEYS * HD, ok ? vsrc + i * RL * vss : vc + (long long)k0 * vss, ok ? 16u : 0u);
+#pragma unroll
+      for (int i = 0; i < CD_KEYS / RL; ++i) {
+        const int key = base + cr + i * RL;
+        const bool ok = key >= k0 && key < k1;
+        const uint32_t off = dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD;
+        cp_async_16(off, ok ? ksrc + i * RL * kss : kc + (long long)k0 * kss, ok ? 16u : 0u);
+        cp_async_16(off + CD_KEYS * HD, ok ? vsrc + i * RL * vss : vc + (long long)k0 * vss, ok ? 16u : 0u);
+      }
     }
   };
 #pragma unroll
@@ -276,6 +300,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
           if (key < k0 || key >= k1) s[q][2 * e] = s[q][2 * e + 1] = -INFINITY;
         }
     }
+    // the maxima move seldom: only when some lane's own maximum is above them do the
+    // lanes agree on new ones and is the state brought to them
     float mx[2], rx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -286,15 +312,15 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
         mx[h] = fmaxf(mx[h], x);
         rx[h] = fmaxf(rx[h], x + ve[q]);
       }
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) {
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], d));
-        rx[h] = fmaxf(rx[h], __shfl_xor_sync(0xffffffffu, rx[h], d));
-      }
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || rx[0] > r[0] || rx[1] > r[1])) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], d));
+          rx[h] = fmaxf(rx[h], __shfl_xor_sync(0xffffffffu, rx[h], d));
+        }
         const float mn = fmaxf(m[h], mx[h]), rn = fmaxf(r[h], rx[h]);
         const float am = m[h] == mn ? 1.f : fast_exp2(m[h] - mn), ar = r[h] == rn ? 1.f : fast_exp2(r[h] - rn);
         m[h] = mn;
@@ -459,11 +485,26 @@ __global__ void __launch_bounds__(MG_THREADS) cache_merge_kernel(const __grid_co
   }
 }
 
+// Raises the kernel's dynamic shared memory limit on the current device, once per
+// device (the attribute stays set).
+template <int HD, int FMT>
+static cudaError_t allow_smem(int smem) {
+  constexpr int kDevices = 64;
+  static std::atomic<bool> done[kDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kDevices && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(cache_decode_kernel<HD, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < kDevices) done[dev].store(true, std::memory_order_release);
+  return e;
+}
+
 template <int HD, int FMT>
 static cudaError_t decode_as(const CacheDecodeParams& p, cudaStream_t stream) {
   constexpr int smem = cd_smem<HD>();
   auto kernel = cache_decode_kernel<HD, FMT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<HD, FMT>(smem);
   if (e != cudaSuccess) return e;
   for (int which = 0; which < 2; ++which)
     if (p.out[which])

@@ -62,6 +62,7 @@ class QuantizedKV:
         self.format = _FORMATS[k.dtype]
         self.batch, self.n_kv_heads, self.capacity, self.head_dim = b, Hkv, cap, d
         self.device = k.device
+        self.index = k.device.index if k.device.type == "cuda" else None
         # the C ABI's argument structs with this cache filled in; each call copies one
         self._write_args, self._read_args, self._decode_args = CacheWriteArgs(), CacheReadArgs(), CacheDecodeArgs()
         for a in (self._write_args, self._read_args, self._decode_args):

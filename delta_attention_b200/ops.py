@@ -15,7 +15,6 @@ caller synchronises anyway) and raises ``DtaError(DTA_ERR_KERNEL_TIMEOUT)``.
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -323,12 +322,16 @@ def _decode_workspace(nbytes: int, device) -> torch.Tensor:
     runs once per layer and token, so a fresh allocation per call would cost
     more host time than the kernel.  Calls on one stream are ordered, so they
     may share it.  (During CUDA graph capture a private buffer is used.)"""
+    return _stream_workspace(nbytes, _device_index(device), _stream())
+
+
+def _stream_workspace(nbytes: int, index: int, stream: int) -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():
-        return _workspace(nbytes, device)
-    key = (_device_index(device), _stream())
+        return _workspace(nbytes, torch.device("cuda", index))
+    key = (index, stream)
     ws = _decode_ws.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _workspace(nbytes, device)
+        ws = _workspace(nbytes, torch.device("cuda", index))
         _decode_ws[key] = ws
     return ws
 
@@ -439,43 +442,46 @@ def backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
 _CACHE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _on_cache_device(op):
-    """Run an op with its cache's device current: its launches, its stream and
-    its workspace then belong to that device."""
-
-    @functools.wraps(op)
-    def call(*args, **kw):
-        cache = next((x for x in args if isinstance(x, QuantizedKV)), None) or kw.get("cache")
-        if cache is None:
-            raise TypeError(f"{op.__name__} needs a QuantizedKV cache")
-        if cache.device.type != "cuda":
-            raise ValueError("delta_attention_b200 ops take CUDA tensors (there is no CPU path)")
-        if cache.device.index == torch.cuda.current_device():
-            return op(*args, **kw)
-        with torch.cuda.device(cache.device):
-            return op(*args, **kw)
-
-    return call
+def _on_cache_device(op, cache, *args, **kw):
+    """Run an op again with its cache's device current (its launches, stream and
+    workspace then belong to that device)."""
+    if cache.device.type != "cuda":
+        raise ValueError("delta_attention_b200 ops take CUDA tensors (there is no CPU path)")
+    with torch.cuda.device(cache.device):
+        return op(*args, **kw)
 
 
-def _device_list(t: torch.Tensor, what: str, cache: QuantizedKV) -> torch.Tensor:
+def _is_current(cache: QuantizedKV) -> bool:
+    return cache.index is not None and cache.index == torch.cuda.current_device()
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of a device as an integer, without a Stream object:
+    these ops run once per layer and token, and building one costs as much
+    host time (3 us) as launching a kernel."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _device_list(t: torch.Tensor, what: str, cache: QuantizedKV) -> int:
     if t.dtype != torch.int32 or t.device != cache.device or t.numel() not in (1, cache.batch) or \
             not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of 1 or {cache.batch} elements on {cache.device}")
-    return t
+    return t.data_ptr()
 
 
-def _cache_source(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [b, h, s, d] if a kernel can read it in place (d contiguous, base
-    and strides multiples of 16 bytes), else an aligned copy."""
-    size, st = t.element_size(), t.stride()
-    if st[3] != 1 or t.data_ptr() % 16 or any(
-            n > 1 and (s <= 0 or s * size % 16) for n, s in zip(t.shape, st[:3])):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+def _in_place(t: torch.Tensor):
+    """(tensor, strides) of ``t`` [b, h, s, d] as a kernel can read it: ``t`` itself
+    where d is contiguous and its base and strides are multiples of 16 bytes,
+    else an aligned copy; a size-1 axis gets a harmless legal stride."""
+    b, h, s, d = t.shape
+    sb, sh, ss, sd = t.stride()
+    sb, sh, ss = sb if b > 1 else d, sh if h > 1 else d, ss if s > 1 else d
+    if sd == 1 and sb > 0 and sh > 0 and ss > 0 and not (sb | sh | ss) * t.element_size() & 15 \
+            and not t.data_ptr() & 15:
+        return t, sb, sh, ss
+    return t.clone(memory_format=torch.contiguous_format), h * s * d, s * d, d
 
 
-@_on_cache_device
 def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, lengths: Optional[torch.Tensor] = None,
                 check: bool = False) -> None:
     """Write ``k``, ``v`` [b, Hkv, s, d] (bf16, fp16 or fp32, post-RoPE) into an
@@ -490,6 +496,8 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, le
     A device position or length outside the cache writes nothing of that
     sequence and is recorded in the error word (:func:`check_errors`;
     ``check=True`` does that right after the launch)."""
+    if not _is_current(cache):
+        return _on_cache_device(cache_write, cache, cache, k, v, pos=pos, lengths=lengths, check=check)
     if k.shape != v.shape or k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (
             cache.batch, cache.n_kv_heads, cache.head_dim):
         raise ValueError(f"k and v must be [{cache.batch}, {cache.n_kv_heads}, s, {cache.head_dim}], got "
@@ -501,26 +509,27 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, le
     s = k.shape[2]
     if s == 0:
         return
-    k, v = _cache_source(k), _cache_source(v)
     a = CacheWriteArgs.from_buffer_copy(cache._write_args)
     a.n_new, a.src_type = s, _CACHE_TYPES[k.dtype]
     if isinstance(pos, torch.Tensor):
-        a.pos_dev, a.n_pos = _device_list(pos, "pos", cache).data_ptr(), pos.numel()
+        a.pos_dev, a.n_pos = _device_list(pos, "pos", cache), pos.numel()
     else:
-        a.pos = int(pos)
-        if not 0 <= a.pos <= cache.capacity - s:
+        pos = int(pos)
+        if not 0 <= pos <= cache.capacity - s:
             raise ValueError(f"positions [{pos}, {pos + s}) are outside the cache of {cache.capacity}")
+        a.pos = pos
     if lengths is not None:
-        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache).data_ptr(), lengths.numel()
-    a.k_new, (a.k_new_stride_b, a.k_new_stride_h, a.k_new_stride_s) = k.data_ptr(), _strides(k)
-    a.v_new, (a.v_new_stride_b, a.v_new_stride_h, a.v_new_stride_s) = v.data_ptr(), _strides(v)
-    a.error_word = error_word(cache.device).data_ptr()
-    _check_status(lib().dta_cache_write(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_write")
+        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache), lengths.numel()
+    k, a.k_new_stride_b, a.k_new_stride_h, a.k_new_stride_s = _in_place(k)
+    v, a.v_new_stride_b, a.v_new_stride_h, a.v_new_stride_s = _in_place(v)
+    a.k_new, a.v_new = k.data_ptr(), v.data_ptr()
+    word = _error_words.get(cache.index)
+    a.error_word = (error_word(cache.device) if word is None else word).data_ptr()
+    _check_status(lib().dta_cache_write(ctypes.byref(a), _raw_stream(cache.index)), "dta_cache_write")
     if check:
         check_errors(cache.device)
 
 
-@_on_cache_device
 def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int = 0,
                lengths: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -529,6 +538,10 @@ def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int =
     fp16 or fp32), each value rounded once.  ``lengths`` (device int32, 1 or b
     elements) are the live key counts: rows at or behind them come back as
     zeros.  ``out`` takes the result instead of new tensors."""
+    if not _is_current(cache):
+        return _on_cache_device(cache_read, cache, cache, n_keys=n_keys, start=start, lengths=lengths, dtype=dtype,
+                                out=out)
+    start = int(start)
     n = cache.capacity - start if n_keys is None else int(n_keys)
     if start < 0 or n < 0 or start + n > cache.capacity:
         raise ValueError(f"positions [{start}, {start + n}) are outside the cache of {cache.capacity}")
@@ -545,15 +558,14 @@ def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int =
     if n == 0:
         return out
     a = CacheReadArgs.from_buffer_copy(cache._read_args)
-    a.start, a.n_keys, a.dst_type = int(start), n, _CACHE_TYPES[dtype]
+    a.start, a.n_keys, a.dst_type = start, n, _CACHE_TYPES[dtype]
     a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
     if lengths is not None:
-        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache).data_ptr(), lengths.numel()
-    _check_status(lib().dta_cache_read(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_read")
+        a.lengths, a.n_lengths = _device_list(lengths, "lengths", cache), lengths.numel()
+    _check_status(lib().dta_cache_read(ctypes.byref(a), _raw_stream(cache.index)), "dta_cache_read")
     return out
 
 
-@_on_cache_device
 def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int, scaling: Optional[float] = None,
                  want_dense: bool = True, want_sparse: bool = True, n_keys: Optional[int] = None,
                  n_keys_dev: Optional[torch.Tensor] = None,
@@ -564,6 +576,10 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     ``n_keys_dev`` (device int32, 1 or b elements) gives the live counts on the
     device instead, at most ``n_keys``, which then sizes the launch.  A
     sequence without keys gets zeros."""
+    if not _is_current(cache):
+        return _on_cache_device(cache_decode, cache, q, cache, window=window, sink=sink, scaling=scaling,
+                                want_dense=want_dense, want_sparse=want_sparse, n_keys=n_keys,
+                                n_keys_dev=n_keys_dev)
     b, H, one, d = q.shape
     if one != 1:
         raise ValueError("cache_decode takes one query row per (batch, head)")
@@ -576,20 +592,24 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     n = cache.capacity if n_keys is None else int(n_keys)
     if not 0 <= n <= cache.capacity:
         raise ValueError(f"n_keys {n} is outside the cache of {cache.capacity}")
-    q = _cache_source(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
-    dense = torch.empty(b, 1, H, d, dtype=torch.bfloat16, device=q.device) if want_dense else None
-    sparse = torch.empty(b, 1, H, d, dtype=torch.bfloat16, device=q.device) if want_sparse else None
     a = CacheDecodeArgs.from_buffer_copy(cache._decode_args)
+    q, a.q_stride_b, a.q_stride_h, _ = _in_place(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
+    a.q = q.data_ptr()
     a.n_heads, a.n_keys, a.window, a.sink = H, n, int(window), int(sink)
     a.scaling = d ** -0.5 if scaling is None else float(scaling)
-    a.q = q.data_ptr()
-    a.q_stride_b, a.q_stride_h = _strides(q)[:2]
-    a.dense_out, a.sparse_out = _ptr(dense), _ptr(sparse)
+    dense = sparse = None
+    if want_dense:
+        dense = q.new_empty((b, 1, H, d))
+        a.dense_out = dense.data_ptr()
+    if want_sparse:
+        sparse = q.new_empty((b, 1, H, d))
+        a.sparse_out = sparse.data_ptr()
     if n_keys_dev is not None:
-        a.n_keys_dev, a.n_lengths = _device_list(n_keys_dev, "n_keys_dev", cache).data_ptr(), n_keys_dev.numel()
-    ws = _decode_workspace(lib().dta_cache_decode_workspace_size(ctypes.byref(a)), cache.device)
+        a.n_keys_dev, a.n_lengths = _device_list(n_keys_dev, "n_keys_dev", cache), n_keys_dev.numel()
+    L, stream = lib(), _raw_stream(cache.index)
+    ws = _stream_workspace(L.dta_cache_decode_workspace_size(ctypes.byref(a)), cache.index, stream)
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check_status(lib().dta_cache_decode(ctypes.byref(a), ctypes.c_void_p(_stream())), "dta_cache_decode")
+    _check_status(L.dta_cache_decode(ctypes.byref(a), stream), "dta_cache_decode")
     return dense, sparse
 
 

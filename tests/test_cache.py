@@ -60,15 +60,13 @@ def test_handle_refuses_sizes():
         QuantizedKV.allocate(1, 1, 16, 64, block=0, device="cpu")
 
 
-def test_ops_refuse_cpu_tensors_and_missing_caches():
+def test_ops_refuse_cpu_tensors():
     c = QuantizedKV(**_tensors())
     x = torch.zeros(2, 3, 1, 64)
     for call in (lambda: ops.cache_write(c, x, x, pos=0), lambda: ops.cache_read(c),
                  lambda: ops.cache_decode(x, c, window=1, sink=1), lambda: ops.cache_read(cache=c)):
         with pytest.raises(ValueError, match="CUDA tensors"):
             call()
-    with pytest.raises(TypeError, match="QuantizedKV"):
-        ops.cache_decode(x, x, window=1, sink=1)
 
 
 def _args(kind):
