@@ -36,17 +36,33 @@ __device__ __forceinline__ int cache_need(float amax) {
   return max(u, 1);
 }
 
-// Four scaled values -> four codes (value 0 in the low byte); ties to even.
+// a * b elementwise (one instruction for two products).
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b));
+  return r;
+}
+
+// Four finite values times a power of two -> four codes (value 0 in the low byte),
+// ties to even; the products lie within the format.
 template <int FMT>
-__device__ __forceinline__ uint32_t cache_pack4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t cache_pack4(float2 a, float2 b, float inv) {
   if constexpr (FMT == CACHE_E4M3) {
+    a = mul2(a, inv);
+    b = mul2(b, inv);
     uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
     return (uint32_t)lo | ((uint32_t)hi << 16);
   } else {
-    const int ia = __float2int_rn(a), ib = __float2int_rn(b), ic = __float2int_rn(c), id = __float2int_rn(d);
-    return (uint32_t)(ia & 255) | ((uint32_t)(ib & 255) << 8) | ((uint32_t)(ic & 255) << 16) | ((uint32_t)id << 24);
+    // x * inv is exact, so x * inv + 1.5 * 2^23 rounds it once, to an integer in the low bits
+    const float magic = 12582912.f;
+    const uint32_t x = __float_as_uint(fmaf(a.x, inv, magic)), y = __float_as_uint(fmaf(a.y, inv, magic));
+    const uint32_t z = __float_as_uint(fmaf(b.x, inv, magic)), w = __float_as_uint(fmaf(b.y, inv, magic));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
   }
 }
 
