@@ -138,6 +138,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
   const int b = blockIdx.y, slab = blockIdx.x / p.Hkv, h = blockIdx.x - slab * p.Hkv;
   const int side = blockIdx.z;
   const CacheSide& S = p.side[side];
+  grid_dependency_wait();
+  grid_dependents_launch();
   // [first, end): the positions that this call writes in sequence b
   const int first = p.pos_dev ? p.pos_dev[b * p.pos_step] : p.pos;
   const int len = p.lengths ? p.lengths[b * p.len_step] : p.n_new;
@@ -251,6 +253,8 @@ __global__ void __launch_bounds__(READ_THREADS) cache_read_kernel(const __grid_c
   const CacheSide& S = p.side[blockIdx.z];
   const uint8_t* codes = S.codes + (long long)b * S.sb + (long long)h * S.sh;
   const uint8_t* scale = S.scale + (long long)b * S.scale_sb + (long long)h * S.scale_sh;
+  grid_dependency_wait();
+  grid_dependents_launch();
   const int live = p.lengths ? p.lengths[b * p.len_step] : p.start + p.n;
   const int ch = threadIdx.x % RC;
   const int r0 = blockIdx.x * (READ_THREADS * READ_CHUNKS / RC) + threadIdx.x / RC;
@@ -302,6 +306,23 @@ __global__ void __launch_bounds__(READ_THREADS) cache_read_kernel(const __grid_c
   }
 }
 
+// Launches as a programmatic dependent: the kernel's CTAs may come up while the last
+// kernel on the stream drains, and wait for it before they touch memory.
+template <typename P>
+static cudaError_t launch_dependent(void (*kernel)(P), dim3 grid, int threads, int smem, cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int HD, int FMT, int SRC>
 static cudaError_t write_as(const CacheWriteParams& p, int batch, cudaStream_t stream) {
   const int T = 1 << p.log_block, group = T * HD / 64;
@@ -314,17 +335,15 @@ static cudaError_t write_as(const CacheWriteParams& p, int batch, cudaStream_t s
         cudaFuncSetAttribute(cache_write_kernel<HD, FMT, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  cache_write_kernel<HD, FMT, SRC>
-      <<<dim3((blocks + per_cta - 1) / per_cta * p.Hkv, batch, 2), threads, smem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(cache_write_kernel<HD, FMT, SRC>,
+                          dim3((unsigned)((blocks + per_cta - 1) / per_cta) * p.Hkv, batch, 2), threads, smem, stream, p);
 }
 
 template <int HD, int FMT, int DST>
 static cudaError_t read_as(const CacheReadParams& p, int batch, cudaStream_t stream) {
   constexpr int rows = READ_THREADS * READ_CHUNKS / (HD / 8);  // per CTA
-  cache_read_kernel<HD, FMT, DST>
-      <<<dim3((p.n + rows - 1) / rows, batch * p.Hkv, 2), READ_THREADS, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(cache_read_kernel<HD, FMT, DST>, dim3((p.n + rows - 1) / rows, batch * p.Hkv, 2), READ_THREADS,
+                          0, stream, p);
 }
 
 #define DTA_CACHE_DISPATCH(FN)                                                       \

@@ -63,6 +63,7 @@ struct CacheDecodeParams {
   int len_step;
   float scale_log2;
   int window, sink;
+  int clusters;            // whether chunks may merge within a cluster
   CacheDecodeSet set[2];   // 0: dense, 1: sparse
   __nv_bfloat16* out[2];   // dense, sparse; either may be null
 };

@@ -50,14 +50,61 @@ int check_list(const int32_t* list, int n, int batch, int* step) {
   return DTA_OK;
 }
 
-// Chunk lengths of the dense set: as many chunks as there are CTAs resident at
-// once (kDenseCtasPerSm per SM), at least kDenseChunkMin keys each.
-#ifndef DTA_CD_CTAS
-#define DTA_CD_CTAS 2
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// Chunk of the sparse set: the shortest multiple of kChunkStep whose sink and window
+// chunks number at most kSparseTarget, up to kSparseChunkMax (they then merge within a
+// cluster: one launch for a sparse-only step); beyond, kSparseChunk.  A function of
+// (sink, window) only, so that a sparse row is the same whichever call it comes from.
+#ifndef DTA_CD_SPARSE_TARGET
+#define DTA_CD_SPARSE_TARGET 9
 #endif
-constexpr int kDenseCtasPerSm = DTA_CD_CTAS;
-constexpr int kDenseChunkMin = 256;
-constexpr int kSparseChunk = 256;
+constexpr int kChunkStep = 128;  // one step of a CTA's warps
+constexpr int kSparseTarget = DTA_CD_SPARSE_TARGET, kSparseChunkMax = 512, kSparseChunk = 256,
+              kSparseChunks = 2048;
+
+int sparse_chunk(long long sink, long long window) {
+  for (int c = kChunkStep; c <= kSparseChunkMax; c += kChunkStep)
+    if (ceil_div(sink, c) + ceil_div(window, c) <= kSparseTarget) return c;
+  // (a launch has at most 65535 chunks: a window of millions of keys gets longer ones)
+  const long long c = ceil_div(ceil_div(sink + window, kSparseChunks), kChunkStep) * kChunkStep;
+  return (int)(c > kSparseChunk ? c : kSparseChunk);
+}
+
+// Chunk of the dense set: the one with the least estimated time.  With `slots` CTAs
+// resident at once, w waves of them take k = w slots / units chunks of each unit (a
+// (batch, KV head)), and cost w times a chunk's steps plus kRampSteps for a CTA's
+// start and end (a step takes 1.5 us while the memory is saturated).  The
+// slots are shared with the sparse set in proportion to the keys, whether it is
+// wanted or not, so that a dense row is the same either way; the sparse chunks then
+// fill the slots that the dense ones leave.  Where sequences have lengths of their
+// own, about half of the chunks are taken to be empty.  `slots` 0: the shortest
+// chunk that any device gets.
+#ifndef DTA_CD_RAMP
+#define DTA_CD_RAMP 3
+#endif
+constexpr int kRampSteps = DTA_CD_RAMP, kWaves = 8;
+
+int dense_chunk(long long n, long long sparse_keys, long long units, bool ragged, long long slots) {
+  if (slots <= 0 || n <= kChunkStep) return kChunkStep;
+  slots = slots * n / (n + sparse_keys);
+  long long best = 0, best_cost = 0;
+  for (int w = 1; w <= kWaves; ++w) {
+    const long long k = w * slots / units > 0 ? w * slots / units : 1;
+    const long long steps = ceil_div(n, k * kChunkStep);
+    const long long chunks = ceil_div(n, steps * kChunkStep) * units;
+    const long long waves = ragged ? ceil_div(chunks, 2 * slots) : ceil_div(chunks, slots);
+    const long long cost = waves * (steps + kRampSteps);
+    if (best == 0 || cost < best_cost) {
+      best = steps * kChunkStep;
+      best_cost = cost;
+    }
+  }
+  return (int)best;
+}
+
+// CTAs of the partial kernel that are resident on an SM (shared memory bounds them).
+int resident_ctas(int head_dim) { return head_dim == 128 ? 2 : 4; }
 
 int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
   if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
@@ -77,16 +124,16 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   p->window = a->window < a->n_keys ? a->window : a->n_keys;
   p->sink = a->sink < a->n_keys ? a->sink : a->n_keys;
   const long long units = (long long)c.batch * c.n_kv_heads, n = a->n_keys;
-  long long chunk = kDenseChunkMin;
-  if (sms > 0) {
-    const long long want = (units * n + (long long)sms * kDenseCtasPerSm - 1) / ((long long)sms * kDenseCtasPerSm);
-    if (want > chunk) chunk = (want + 63) / 64 * 64;
-  }
-  p->set[0].chunk = (int)chunk;
-  p->set[0].n_launched = (int)((n + chunk - 1) / chunk);
-  p->set[1].chunk = kSparseChunk;
-  p->set[1].n_sink_chunks = (p->sink + kSparseChunk - 1) / kSparseChunk;
-  p->set[1].n_launched = p->set[1].n_sink_chunks + (p->window + kSparseChunk - 1) / kSparseChunk;
+  const long long sparse_keys = p->sink + (long long)p->window;
+  const bool ragged = p->n_keys_dev && p->len_step;
+  p->set[0].chunk = dense_chunk(n, sparse_keys < n ? sparse_keys : n, units, ragged,
+                                (long long)sms * resident_ctas(c.head_dim));
+  p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
+  p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
+  const int sc = sparse_chunk(p->sink, p->window);
+  p->set[1].chunk = sc;
+  p->set[1].n_sink_chunks = (int)ceil_div(p->sink, sc);
+  p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, sc);
   for (dta::CacheDecodeSet& S : p->set)
     if (S.n_launched < 1) S.n_launched = 1;  // no keys: one empty partial
   return DTA_OK;

@@ -13,13 +13,14 @@
 //
 // Split-K over the cache: CTA (chunk, batch x KV head) reads its chunk's codes once
 // for all G <= 8 query heads of the group; the partials (m, l, r, o) of the chunks
-// are merged by a second, dependent launch.
+// are merged within a thread-block cluster or by a second, dependent launch.
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "dta_cache.h"
 #include "dta_cache_codes.cuh"
@@ -87,6 +88,52 @@ __device__ __forceinline__ void cd_range(const CacheDecodeParams& p, const Cache
   k1 = max(k1, k0);
 }
 
+// Merging partials (m, l, r, o) of chunks by the log-sum-exp rule.  The lanes of a
+// warp hold the headers (32 per array element); every lane ends up with the total.
+constexpr int MG_ROWS = 4, MG_LOADS = 16;
+template <int HEADS>
+struct MergeState {
+  float M, R, L;
+  __device__ __forceinline__ void start() {
+    M = R = -INFINITY;
+    L = 0.f;
+  }
+  // Takes more chunks: wo their factors on o (0 for a chunk without keys); returns
+  // the factor that brings the o of earlier chunks to the new maximum.
+  __device__ __forceinline__ float weigh(const float (&m)[HEADS], const float (&l)[HEADS], const float (&r)[HEADS],
+                                         float (&wo)[HEADS]) {
+    float mt = M, rt = R;
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+      mt = fmaxf(mt, m[k]);
+      rt = fmaxf(rt, r[k]);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x /= 2) {
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+      rt = fmaxf(rt, __shfl_xor_sync(0xffffffffu, rt, x));
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+      sum += l[k] == 0.f ? 0.f : l[k] * fast_exp2(m[k] - mt);
+      wo[k] = l[k] == 0.f ? 0.f : fast_exp2(r[k] - rt);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    L = (M == mt ? L : L * fast_exp2(M - mt)) + sum;
+    const float f = R == rt ? 1.f : fast_exp2(R - rt);
+    M = mt;
+    R = rt;
+    return f;
+  }
+  __device__ __forceinline__ __nv_bfloat16 finish(float o) const {
+    return __float2bfloat16_rn(L == 0.f ? 0.f : (o * 0x1p-14f) * exp2f(R - M) / L);
+  }
+};
+__device__ __forceinline__ void merge_add(float& acc, float o, float w) { acc = w == 0.f ? acc : fmaf(o, w, acc); }
+constexpr int CD_CLUSTER_MAX = 16;  // CTAs of a cluster (above 8: non-portable sizes, used where they fit)
+
 // Shared-memory ring of one warp: CD_STAGES stages of CD_KEYS keys, each K rows
 // then V rows of HD bytes.  The 16-byte pieces of row r are permuted by r, so
 // that the fragment reads below are free of bank conflicts (HD = 128; at 64 the
@@ -117,18 +164,36 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
 //                                     tile j are dims HD/8 g + 2j and + 1
 // so that codes go from shared memory into fragments without any exchange; only
 // the weights are transposed (movmatrix).
-template <int HD, int FMT>
-__global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_constant__ CacheDecodeParams p, int which) {
+//
+// The grid's y covers the dense set's chunks and then the sparse set's, so a call
+// that wants both rows is one launch, whose short sparse chunks start last (and find
+// the sink and window in L2); its x the (batch, KV head) pairs.  CLU: the y extent is
+// one thread-block cluster per pair, and the
+// cluster merges its chunks' partials through distributed shared memory; else they
+// go to global memory and cache_merge_kernel merges them.  Both merge in one order,
+// so a sparse row is the same bit for bit whichever way it was launched.
+template <int HD, int FMT, bool CLU>
+__global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_constant__ CacheDecodeParams p) {
   constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16, NG = CD_KEYS / CACHE_GROUP;
   extern __shared__ __align__(128) uint8_t cd_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.y / p.Hkv, hk = blockIdx.y - b * p.Hkv;
+  const int b = blockIdx.x / p.Hkv, hk = blockIdx.x - b * p.Hkv;
   const int G = p.G;
+  const int n_dense = p.out[0] ? p.set[0].n_launched : 0;
+  const int which = (int)blockIdx.y < n_dense ? 0 : 1, chunk = blockIdx.y - (which ? n_dense : 0);
   const CacheDecodeSet& S = p.set[which];
-  grid_dependents_launch();
+  grid_dependency_wait();    // launched as a programmatic dependent of whatever ran before
+  grid_dependents_launch();  // (the merge launch, which waits for this grid in turn)
   int k0, k1;
-  cd_range(p, S, which, cd_live(p, b), blockIdx.x, k0, k1);
+  cd_range(p, S, which, cd_live(p, b), chunk, k0, k1);
+
+  if (!CLU && k0 >= k1) {  // no keys: an empty partial (its o is not read)
+    if (threadIdx.x < G)
+      *reinterpret_cast<float4*>(S.partials + ((long long)(b * p.H + hk * G + threadIdx.x) * S.n_launched + chunk) * (4 + HD)) =
+          make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    return;
+  }
 
   const uint8_t* kc = p.side[0].codes + (long long)b * p.side[0].sb + (long long)hk * p.side[0].sh;
   const uint8_t* vc = p.side[1].codes + (long long)b * p.side[1].sb + (long long)hk * p.side[1].sh;
@@ -394,7 +459,11 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     }
   }
   __syncthreads();
-  float* part0 = S.partials + ((long long)(b * p.H + hk * G) * S.n_launched + blockIdx.x) * (4 + HD);
+  // this chunk's partial: to global memory, or (CLU) to own[8][4 + HD]
+  float* own = red_s + CD_WARPS * 24;
+  const long long hstride = CLU ? 4 + HD : (long long)S.n_launched * (4 + HD);
+  float* part0 =
+      CLU ? own : S.partials + ((long long)(b * p.H + hk * G) * S.n_launched + chunk) * (4 + HD);
   for (int idx = threadIdx.x; idx < G * HD; idx += CD_THREADS) {
     const int h = idx / HD, d = idx - h * HD;
     float M = -INFINITY, R = -INFINITY;
@@ -410,7 +479,7 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       L += red_s[w * 24 + 8 + h] * fast_exp2(red_s[w * 24 + h] - M);
       O += red_o[(w * 8 + h) * HD + d] * fast_exp2(red_s[w * 24 + 16 + h] - R);
     }
-    float* part = part0 + (long long)h * S.n_launched * (4 + HD);
+    float* part = part0 + h * hstride;
     part[4 + d] = O;
     if (d == 0) {
       part[0] = M;
@@ -418,102 +487,172 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       part[2] = R;
     }
   }
+  if constexpr (CLU) {
+    static_assert(cd_smem<HD>() >= (CD_WARPS * 8 * HD + CD_WARPS * 24 + 8 * (4 + HD)) * 4, "partial fits behind them");
+    __syncwarp();
+    cluster_sync();
+    // items of 32 columns of one row of one set, dealt to the cluster's warps
+    constexpr int COLS = HD / 32;
+    const int nct = (int)cluster_nctarank();
+    const int sets = (p.out[0] ? 1 : 0) + (p.out[1] ? 1 : 0);
+    const uint32_t mine = smem_u32(own);
+    for (int item = (int)cluster_ctarank() * CD_WARPS + warp; item < sets * G * COLS; item += nct * CD_WARPS) {
+      const int set = p.out[0] ? item / (G * COLS) : 1, row = item / COLS % G, d = item % COLS * 32 + lane;
+      const int r0 = set ? n_dense : 0, n = p.set[set].n_launched;
+      const uint32_t at = mine + row * (4 + HD) * 4;
+      float ov[CD_CLUSTER_MAX];
+#pragma unroll
+      for (int x = 0; x < CD_CLUSTER_MAX; ++x)
+        ov[x] = x < n ? ld_dsmem_f32(dsmem_addr(at + (4 + d) * 4, r0 + x)) : 0.f;
+      float hm = -INFINITY, hl = 0.f, hr = -INFINITY;
+      if (lane < n) {
+        const uint32_t head = dsmem_addr(at, r0 + lane);
+        hm = ld_dsmem_f32(head);
+        hl = ld_dsmem_f32(head + 4);
+        hr = ld_dsmem_f32(head + 8);
+      }
+      MergeState<1> st;
+      st.start();
+      const float hms[1] = {hm}, hls[1] = {hl}, hrs[1] = {hr};
+      float wo[1];
+      st.weigh(hms, hls, hrs, wo);
+      float acc[MG_ROWS] = {};
+#pragma unroll
+      for (int x = 0; x < CD_CLUSTER_MAX; ++x) merge_add(acc[x % MG_ROWS], ov[x], __shfl_sync(0xffffffffu, wo[0], x));
+#pragma unroll
+      for (int y = 1; y < MG_ROWS; ++y) acc[0] += acc[y];
+      p.out[set][(long long)(b * p.H + hk * G + row) * HD + d] = st.finish(acc[0]);
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA exits while a peer may still read its partial
+  }
 }
 
-// Merge of a key set's partials: grid (B * H, key sets), MG_THREADS / HD threads per
-// head dim.  The threads' columns of the first MG_THREADS / HD * MG_LOADS chunks are on their
-// way while the chunks' weights are formed, so a set of up to that many chunks
-// costs one round trip to L2.  A programmatic dependent launch: its CTAs are
-// resident when the partials' grid ends.
-constexpr int MG_THREADS = 512, MG_LOADS = 8;
-
+// Merge of a key set's partials: grid (B * H, key sets), MG_ROWS threads per head
+// dim.  The threads' columns of the first MG_ROWS * MG_LOADS chunks and their headers
+// are fetched at once, so a set of up to that many chunks costs one round trip to L2.
+// A programmatic dependent launch: its CTAs are resident when the partials' grid ends.
 template <int HD>
-__global__ void __launch_bounds__(MG_THREADS) cache_merge_kernel(const __grid_constant__ CacheDecodeParams p) {
-  constexpr int ROWS = MG_THREADS / HD, TILE = ROWS * MG_LOADS;
-  __shared__ float wl[TILE], wo[TILE], hm[TILE], hr[TILE];
-  __shared__ float red[ROWS][HD];
+__global__ void __launch_bounds__(MG_ROWS* HD) cache_merge_kernel(const __grid_constant__ CacheDecodeParams p) {
+  constexpr int TILE = MG_ROWS * MG_LOADS, HEADS = TILE / 32;
+  static_assert(HD % 32 == 0 && TILE % 32 == 0, "a warp's lanes hold one tile's headers and share a row");
+  __shared__ float red[MG_ROWS][HD];
   const int bh = blockIdx.x, which = p.out[0] ? blockIdx.y : 1;
-  const int d = threadIdx.x % HD, y = threadIdx.x / HD;
+  const int d = threadIdx.x % HD, y = threadIdx.x / HD, lane = threadIdx.x & 31;
   const CacheDecodeSet& S = p.set[which];
   const float* base = S.partials + (long long)bh * S.n_launched * (4 + HD);
   grid_dependency_wait();
-  float M = -INFINITY, R = -INFINITY, L = 0.f, O = 0.f;
+  MergeState<HEADS> st;
+  st.start();
+  float O = 0.f;
   for (int x0 = 0; x0 < S.n_launched; x0 += TILE) {
     const int n = min(TILE, S.n_launched - x0);
     const float* tile = base + (long long)x0 * (4 + HD);
     float ov[MG_LOADS];
 #pragma unroll
     for (int i = 0; i < MG_LOADS; ++i) {
-      const int x = y + i * ROWS;
+      const int x = y + i * MG_ROWS;
       ov[i] = x < n ? tile[(long long)x * (4 + HD) + 4 + d] : 0.f;
     }
-    float l = 0.f;
-    if (threadIdx.x < TILE) {
-      float4 h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-      if ((int)threadIdx.x < n) h = *reinterpret_cast<const float4*>(tile + (long long)threadIdx.x * (4 + HD));
-      l = h.y;
-      hm[threadIdx.x] = h.x;
-      hr[threadIdx.x] = h.z;
-    }
-    __syncthreads();
-    float mt = M, rt = R;
-    for (int x = 0; x < n; ++x) {
-      mt = fmaxf(mt, hm[x]);
-      rt = fmaxf(rt, hr[x]);
-    }
-    if (threadIdx.x < TILE) {  // a chunk without keys has no weight
-      wl[threadIdx.x] = l == 0.f ? 0.f : l * fast_exp2(hm[threadIdx.x] - mt);
-      wo[threadIdx.x] = l == 0.f ? 0.f : fast_exp2(hr[threadIdx.x] - rt);
-    }
-    __syncthreads();
-    if (M != mt) L *= fast_exp2(M - mt);
-    if (R != rt) O *= fast_exp2(R - rt);
-    M = mt;
-    R = rt;
-    for (int x = 0; x < n; ++x) L += wl[x];
+    float hm[HEADS], hl[HEADS], hr[HEADS], wo[HEADS];
 #pragma unroll
-    for (int i = 0; i < MG_LOADS; ++i) O += wo[y + i * ROWS] == 0.f ? 0.f : ov[i] * wo[y + i * ROWS];
-    __syncthreads();
+    for (int k = 0; k < HEADS; ++k) {
+      const int x = lane + 32 * k;
+      float4 h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      if (x < n) h = *reinterpret_cast<const float4*>(tile + (long long)x * (4 + HD));
+      hm[k] = h.x;
+      hl[k] = h.y;
+      hr[k] = h.z;
+    }
+    O *= st.weigh(hm, hl, hr, wo);
+#pragma unroll
+    for (int i = 0; i < MG_LOADS; ++i)
+      merge_add(O, ov[i], __shfl_sync(0xffffffffu, wo[i * MG_ROWS / 32], (y + i * MG_ROWS) & 31));
   }
   red[y][d] = O;
   __syncthreads();
   if (y == 0) {
 #pragma unroll
-    for (int i = 1; i < ROWS; ++i) O += red[i][d];
-    const float v = L == 0.f ? 0.f : (O * 0x1p-14f) * exp2f(R - M) / L;
-    p.out[which][(long long)bh * HD + d] = __float2bfloat16_rn(v);
+    for (int i = 1; i < MG_ROWS; ++i) O += red[i][d];
+    p.out[which][(long long)bh * HD + d] = st.finish(O);
   }
 }
 
-// Raises the kernel's dynamic shared memory limit on the current device, once per
-// device (the attribute stays set).
-template <int HD, int FMT>
-static cudaError_t allow_smem(int smem) {
+// Sets the kernel's launch attributes on the current device, once per device (they
+// stay set), and for a cluster size asks whether such a cluster can be scheduled.
+template <int HD, int FMT, bool CLU>
+static cudaError_t prepare_kernel(int nct, bool* fits) {
   constexpr int kDevices = 64;
-  static std::atomic<bool> done[kDevices];
+  static std::mutex mu;
+  static std::atomic<int> state[kDevices][CD_CLUSTER_MAX + 1];  // 0 unknown, 1 ready, 2 does not fit
+  auto kernel = cache_decode_kernel<HD, FMT, CLU>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev < kDevices && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
-  e = cudaFuncSetAttribute(cache_decode_kernel<HD, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && dev < kDevices) done[dev].store(true, std::memory_order_release);
-  return e;
+  if (dev < 0 || dev >= kDevices) return cudaErrorInvalidDevice;
+  std::atomic<int>& st = state[dev][CLU ? nct : 0];
+  if (st.load(std::memory_order_acquire) == 0) {
+    std::lock_guard<std::mutex> lock(mu);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cd_smem<HD>());
+    if (e == cudaSuccess && CLU) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    int n = 1;
+    if (CLU) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, nct);
+      cfg.blockDim = dim3(CD_THREADS);
+      cfg.dynamicSmemBytes = cd_smem<HD>();
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.y = nct;
+      attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();  // a refused size is not an error of the call
+        n = 0;
+      }
+    }
+    st.store(n > 0 ? 1 : 2, std::memory_order_release);
+  }
+  *fits = st.load(std::memory_order_acquire) == 1;
+  return cudaSuccess;
+}
+
+template <int HD, int FMT, bool CLU>
+static cudaError_t launch_partials(const CacheDecodeParams& p, int nct, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.B * p.Hkv, nct);
+  cfg.blockDim = dim3(CD_THREADS);
+  cfg.dynamicSmemBytes = cd_smem<HD>();
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.y = nct;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLU ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, cache_decode_kernel<HD, FMT, CLU>, p);
 }
 
 template <int HD, int FMT>
 static cudaError_t decode_as(const CacheDecodeParams& p, cudaStream_t stream) {
-  constexpr int smem = cd_smem<HD>();
-  auto kernel = cache_decode_kernel<HD, FMT>;
-  cudaError_t e = allow_smem<HD, FMT>(smem);
-  if (e != cudaSuccess) return e;
+  int nct = 0;
   for (int which = 0; which < 2; ++which)
-    if (p.out[which])
-      kernel<<<dim3(p.set[which].n_launched, p.B * p.Hkv), CD_THREADS, smem, stream>>>(p, which);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+    if (p.out[which]) nct += p.set[which].n_launched;
+  bool fits = false;
+  cudaError_t e;
+  if (p.clusters && nct <= CD_CLUSTER_MAX) {
+    if ((e = prepare_kernel<HD, FMT, true>(nct, &fits)) != cudaSuccess) return e;
+    if (fits) return launch_partials<HD, FMT, true>(p, nct, stream);
+  }
+  if ((e = prepare_kernel<HD, FMT, false>(0, &fits)) != cudaSuccess) return e;
+  if ((e = launch_partials<HD, FMT, false>(p, nct, stream)) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.B * p.H, (p.out[0] ? 1 : 0) + (p.out[1] ? 1 : 0));
-  cfg.blockDim = dim3(MG_THREADS);
+  cfg.blockDim = dim3(MG_ROWS * HD);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
