@@ -30,10 +30,19 @@ import torch
 
 from . import ops
 from .drift import drift_summary
+from .kv_cache import QuantizedKV
 
 
 def _cfg(config, name, default):
     return getattr(config, name, default)
+
+
+def _decode(q, k, v, n_keys=None, **kw):
+    """``ops.decode`` over 16-bit keys and values, or ``ops.cache_decode`` over
+    the first ``n_keys`` keys of an 8-bit cache (``v`` is then unused)."""
+    if isinstance(k, QuantizedKV):
+        return ops.cache_decode(q, k, n_keys=n_keys, **kw)
+    return ops.decode(q, k, v, **kw)
 
 
 class DeltaAttention(torch.nn.Module):
@@ -96,27 +105,34 @@ class DeltaAttention(torch.nn.Module):
                                dropout: float = 0.0, scaling: float = 1.0, **kwargs):
         """Dense attention of ``s`` new rows over ``n`` cached keys with the
         rectangle mask ``tril(n - s)``; single-token steps go to the
-        sparse/delta decode path when ``decode_mode != "dense"``."""
+        sparse/delta decode path when ``decode_mode != "dense"``.
+        ``key_states`` may be a :class:`QuantizedKV` (``value_states`` is then
+        None) with ``n_keys`` live keys (default: its capacity); several rows
+        then attend over what its prefix reads back as."""
         b, _, s, d = query_states.size()
+        n_keys = kwargs.get("n_keys")
         if s == 1 and _cfg(self.config, "decode_mode", "dense") != "dense":
-            return self.delta_decode_forward(module, query_states, key_states, value_states, scaling=scaling)
-        n = key_states.size(2)
+            return self.delta_decode_forward(module, query_states, key_states, value_states, scaling=scaling,
+                                             n_keys=n_keys)
         if s == 1:
-            dense, _ = ops.decode(query_states, key_states, value_states, window=0, sink=0, scaling=scaling,
-                                  want_dense=True, want_sparse=False)
+            dense, _ = _decode(query_states, key_states, value_states, n_keys, window=0, sink=0, scaling=scaling,
+                               want_dense=True, want_sparse=False)
             return dense, None
+        if isinstance(key_states, QuantizedKV):
+            key_states, value_states = ops.cache_read(key_states, n_keys=n_keys)
+        n = key_states.size(2)
         rows = torch.arange(s, device=query_states.device, dtype=torch.int32)
         out = ops.rows(query_states, key_states, value_states, rows, rows + (n - s), scaling=scaling,
                        validate=False)
         return out, None
 
-    def _decode_sparse_row(self, q, k, v, scaling):
+    def _decode_sparse_row(self, q, k, v, scaling, n_keys=None):
         """StreamingLLM decode row: the first ``sink`` keys plus the last
         ``sliding_window`` keys (all keys when the cache is shorter).
         Returns [b, 1, H, d]."""
-        _, sparse = ops.decode(q, k, v, window=int(self.config.sliding_window),
-                               sink=int(_cfg(self.config, "sink", 1024)), scaling=scaling,
-                               want_dense=False, want_sparse=True)
+        _, sparse = _decode(q, k, v, n_keys, window=int(self.config.sliding_window),
+                            sink=int(_cfg(self.config, "sink", 1024)), scaling=scaling,
+                            want_dense=False, want_sparse=True)
         return sparse
 
     def delta_decode_forward(self, module, query_states, key_states, value_states, scaling=1.0, **kwargs):
@@ -129,16 +145,18 @@ class DeltaAttention(torch.nn.Module):
         the dense row and refresh the delta; other steps output sparse + delta.
         When the anchor decision is known before attention runs (first step,
         cap, fixed policy), the dense and sparse rows come from ONE pass over
-        the cache.  Batch > 1 shares one schedule per layer.
+        the cache.  Batch > 1 shares one schedule per layer.  As in
+        ``sdpa_rectangle_forward``, ``key_states`` may be an 8-bit cache.
         """
         cfg = self.config
+        n_keys = kwargs.get("n_keys")
         mode = cfg.decode_mode
         assert mode in ("sparse", "delta"), mode
         q, k, v = query_states, key_states, value_states
         window = int(cfg.sliding_window)
         sink = int(_cfg(cfg, "sink", 1024))
         if mode == "sparse":
-            return self._decode_sparse_row(q, k, v, scaling), None
+            return self._decode_sparse_row(q, k, v, scaling, n_keys), None
 
         st = self._dec_state or {"last_delta": None, "steps": 0, "last_sparse": None, "cos_hist": []}
         log_drift = bool(_cfg(cfg, "log_drift", False))
@@ -157,8 +175,8 @@ class DeltaAttention(torch.nn.Module):
                 anchor = True
             decided = anchor or policy not in ("drift", "drift_rel") or st["last_sparse"] is None
         want_dense_now = (decided and anchor) or log_drift
-        dense_out, sparse_out = ops.decode(q, k, v, window=window, sink=sink, scaling=scaling,
-                                           want_dense=want_dense_now, want_sparse=True)
+        dense_out, sparse_out = _decode(q, k, v, n_keys, window=window, sink=sink, scaling=scaling,
+                                        want_dense=want_dense_now, want_sparse=True)
         if not decided:
             c = _cos(sparse_out, st["last_sparse"])
             if policy == "drift":
@@ -172,8 +190,8 @@ class DeltaAttention(torch.nn.Module):
                 hist.append(c)
                 del hist[:-16]
             if anchor and dense_out is None:
-                dense_out, _ = ops.decode(q, k, v, window=window, sink=sink, scaling=scaling,
-                                          want_dense=True, want_sparse=False)
+                dense_out, _ = _decode(q, k, v, n_keys, window=window, sink=sink, scaling=scaling,
+                                       want_dense=True, want_sparse=False)
         if anchor:
             st["last_delta"] = dense_out - sparse_out
             st["steps"] = 0

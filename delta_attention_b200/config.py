@@ -2,12 +2,14 @@
 
 Mirrors the hot-path fields of the reference's ``Config`` dataclass
 (``delta_attention/config.py:9-78``) with the same names, defaults and
-meaning, plus two fields the reference hard-codes:
+meaning, plus two fields the reference hard-codes and the decoder's cache format:
 
 * ``sink`` -- attention-sink tokens; the reference fixes 1024
   (``delta_attention/llama.py:415,543``).
 * ``q_block`` -- query block of hip-attn's block-anchored window; the
   reference fixes 64 (``delta_attention/config.py:117,136``).
+* ``kv_cache``, ``kv_block`` -- format of the decoder's KV cache and the tokens per
+  scale of an 8-bit one (no counterpart in the reference).
 
 ``delta_lambda`` keeps the reference's meaning: the integer anchor stride
 (gamma), not a scale factor (``delta_attention/llama.py:651,673``).
@@ -53,6 +55,9 @@ class Config:
     gamma_dec_max: int = 128
 
     max_new_tokens: int = 128
+
+    kv_cache: str = "bf16"                   # KV cache of the decoder: [bf16, e4m3, int8]
+    kv_block: int = 64                       # tokens per scale of an 8-bit cache [16, 32, 64, 128]
 
     @classmethod
     def from_args(cls, argv: Optional[Sequence[str]] = None) -> "Config":

@@ -35,6 +35,7 @@ import torch
 
 from .attention import DeltaAttention
 from .config import PIPELINE_FIELDS, Config
+from .kv_cache import CODE_TYPES, QuantizedKV
 from .rope import cos_sin, rotate_half
 
 
@@ -168,17 +169,32 @@ class DeltaDecoder:
             self.layers.append(layer)
         self.k_cache: List[torch.Tensor] = []
         self.v_cache: List[torch.Tensor] = []
+        self.kv8: List[QuantizedKV] = []  # in place of k_cache and v_cache with an 8-bit cache
         self.length = 0
+        kind = getattr(cfg, "kv_cache", "bf16")
+        if kind != "bf16" and kind not in CODE_TYPES:
+            raise ValueError(f"unknown kv_cache {kind!r} (bf16, {', '.join(CODE_TYPES)})")
+        self.kv_kind = kind
         llama3 = dict(arch.rope_llama3) if arch.rope_llama3 else None
         self._rope = (arch.head_dim, arch.rope_theta, llama3)
 
     # ------------------------------------------------------------------
     def allocate_cache(self, batch: int, max_len: int) -> None:
-        """KV cache [B, KV heads of this rank, max_len, d] per layer, bf16."""
+        """KV cache [B, KV heads of this rank, max_len, d] per layer, bf16 or the
+        8-bit format ``Config.kv_cache`` names."""
         shape = (batch, self.Hkvl, max_len, self.arch.head_dim)
+        self.length = 0
+        if self.kv_kind != "bf16":
+            self.kv8 = [QuantizedKV.allocate(*shape, format=self.kv_kind, block=int(self.cfg.kv_block),
+                                             device=self.device) for _ in self.layers]
+            return
         self.k_cache = [torch.empty(shape, device=self.device, dtype=self.dtype) for _ in self.layers]
         self.v_cache = [torch.empty(shape, device=self.device, dtype=self.dtype) for _ in self.layers]
-        self.length = 0
+
+    def _capacity(self) -> int:
+        if self.kv8:
+            return self.kv8[0].capacity
+        return self.k_cache[0].shape[2] if self.k_cache else 0
 
     def _timed(self, name: str):
         """CUDA-event bracket around one phase of a layer (benchmark only)."""
@@ -187,22 +203,25 @@ class DeltaDecoder:
             return _NullCtx()
         return _EventCtx(ev.setdefault(name, []))
 
-    def _attend(self, i: int, layer, q, k, v, prefill: bool) -> torch.Tensor:
+    def _attend(self, i: int, layer, q, k, v, prefill: bool, **kw) -> torch.Tensor:
         if self.attention is not None:
             return self.attention(i, q, k, v, self.scaling, prefill)
         plug = layer["plugin"]
         if prefill:
             out, _ = plug.delta_forward(plug, q, k, v, None, scaling=self.scaling)
         else:
-            out, _ = plug.sdpa_rectangle_forward(plug, q, k, v, None, scaling=self.scaling)
+            out, _ = plug.sdpa_rectangle_forward(plug, q, k, v, None, scaling=self.scaling, **kw)
         return out
 
     def _layer(self, i: int, x: torch.Tensor, pos0: int, cos: torch.Tensor, sin: torch.Tensor,
-               pos_t: Optional[torch.Tensor] = None, attend: Optional[Callable] = None) -> torch.Tensor:
-        """One decoder layer.  ``pos_t`` (a device position, one new token)
-        and ``attend(i, q, k_cache, v_cache)`` select the graph-replayed decode
-        step: the cache write and the attention then take the position from
-        device memory and the attention reads the whole cache."""
+               pos_t: Optional[torch.Tensor] = None, attend: Optional[Callable] = None,
+               pos32: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One decoder layer.  ``pos_t`` (a device position, one new token; as
+        int32 in ``pos32``) and ``attend(i, q, k_cache, v_cache)`` select the
+        graph-replayed decode step: the cache write and the attention then take
+        the position from device memory and the attention reads the whole
+        cache.  With an 8-bit cache a prompt attends its own keys and values as
+        they are, later rows what the cache holds."""
         a, layer = self.arch, self.layers[i]
         B, s, D = x.shape
         d = a.head_dim
@@ -222,8 +241,21 @@ class DeltaDecoder:
         q = q * c + rotate_half(q) * sn
         k = k * c + rotate_half(k) * sn
         # KV-cache write path: post-RoPE keys and values at positions [pos0, pos0 + s)
-        kc, vc = self.k_cache[i], self.v_cache[i]
-        if pos_t is not None:
+        kc, vc = (self.kv8[i], None) if self.kv8 else (self.k_cache[i], self.v_cache[i])
+        if self.kv8:
+            from . import ops
+
+            k, v = k.transpose(1, 2), v.transpose(1, 2)
+            ops.cache_write(kc, k, v, pos=pos0 if pos_t is None else pos32)
+            if pos_t is not None:
+                o = attend(i, q.transpose(1, 2), kc, vc)
+            else:
+                with self._timed("attention"):
+                    if pos0 == 0:
+                        o = self._attend(i, layer, q.transpose(1, 2), k, v, prefill=True)
+                    else:
+                        o = self._attend(i, layer, q.transpose(1, 2), kc, vc, prefill=False, n_keys=pos0 + s)
+        elif pos_t is not None:
             kc.index_copy_(2, pos_t, k.transpose(1, 2))
             vc.index_copy_(2, pos_t, v.transpose(1, 2))
             o = attend(i, q.transpose(1, 2), kc, vc)
@@ -272,7 +304,7 @@ class DeltaDecoder:
         if pos0 == 0:
             for layer in self.layers:  # a new prompt: no decode state carries over
                 layer["plugin"].reset_decode_state()
-        if pos0 + s > (self.k_cache[0].shape[2] if self.k_cache else 0):
+        if pos0 + s > self._capacity():
             raise ValueError("KV cache too short: call allocate_cache(batch, max_len) first")
         x = self.embed[input_ids.to(self.embed.device)]
         cos, sin = cos_sin(torch.arange(pos0, pos0 + s, device=self.device), *self._rope)
@@ -323,6 +355,7 @@ class DecodeGraph:
         self.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         self.pos = torch.zeros(1, dtype=torch.long, device=dev)
         self.n_keys = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.pos32 = torch.zeros(1, dtype=torch.int32, device=dev)  # pos, for an 8-bit cache's write
         self.hidden = torch.zeros(batch, model.arch.hidden, dtype=model.dtype, device=dev)  # last step's output
         self.delta = [torch.zeros(batch, 1, model.Hl, d, dtype=torch.bfloat16, device=dev) for _ in model.layers] \
             if self.mode == "delta" else []
@@ -336,16 +369,22 @@ class DecodeGraph:
 
         def attend(i, q, kc, vc):
             kw = dict(window=self.window, sink=self.sink, scaling=m.scaling, n_keys_dev=self.n_keys)
+            if m.kv8:
+                def decode(**want):
+                    return ops.cache_decode(q, kc, **want, **kw)
+            else:
+                def decode(**want):
+                    return ops.decode(q, kc, vc, **want, **kw)
             if self.mode == "dense":
-                out, _ = ops.decode(q, kc, vc, want_dense=True, want_sparse=False, **kw)
+                out, _ = decode(want_dense=True, want_sparse=False)
             elif self.mode == "sparse":
-                _, out = ops.decode(q, kc, vc, want_dense=False, want_sparse=True, **kw)
+                _, out = decode(want_dense=False, want_sparse=True)
             elif anchor:
-                dense, sparse = ops.decode(q, kc, vc, want_dense=True, want_sparse=True, **kw)
+                dense, sparse = decode(want_dense=True, want_sparse=True)
                 self.delta[i].copy_(dense - sparse)
                 out = dense
             else:
-                _, sparse = ops.decode(q, kc, vc, want_dense=False, want_sparse=True, **kw)
+                _, sparse = decode(want_dense=False, want_sparse=True)
                 out = sparse + self.delta[i]
             return out
 
@@ -357,14 +396,27 @@ class DecodeGraph:
         cos, sin = cos_sin(self.pos, *m._rope)
         attend = self._attend(anchor)
         for i in range(len(m.layers)):
-            x = m._layer(i, x, 0, cos, sin, pos_t=self.pos, attend=attend)
+            x = m._layer(i, x, 0, cos, sin, pos_t=self.pos, attend=attend, pos32=self.pos32)
         self.hidden.copy_(x[:, -1])
         self.tok.copy_(m._next_token(x[:, -1]))
         self.pos.add_(1)
+        self.pos32.add_(1)
         self.n_keys.add_(1)
 
+    def _state(self) -> List[torch.Tensor]:
+        """What a step advances on the device, but for what the next step
+        writes again: the counters and, with an 8-bit cache, the block that
+        holds the position (a write may raise its scale)."""
+        m, out = self.model, [self.tok, self.pos, self.pos32, self.n_keys]
+        for c in m.kv8:
+            blk = m.length // c.block
+            at = slice(blk * c.block, (blk + 1) * c.block)
+            out += [t.view(torch.uint8) for t in (c.k[:, :, at], c.v[:, :, at], c.k_scale[:, :, blk:blk + 1],
+                                                  c.v_scale[:, :, blk:blk + 1])]
+        return out
+
     def _capture(self) -> None:
-        saved = (self.tok.clone(), self.pos.clone(), self.n_keys.clone())
+        saved = [t.clone() for t in self._state()]
         for anchor in ((True, False) if self.mode == "delta" else (False,)):
             # one eager run first (kernel attributes, library handles, NCCL
             # communicators), then rewind the device state it advanced; the
@@ -374,7 +426,7 @@ class DecodeGraph:
             with torch.cuda.stream(side):
                 self._step(anchor)
             torch.cuda.current_stream().wait_stream(side)
-            for t, v in zip((self.tok, self.pos, self.n_keys), saved):
+            for t, v in zip(self._state(), saved):
                 t.copy_(v)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
@@ -387,6 +439,7 @@ class DecodeGraph:
         m = self.model
         self.tok.copy_(first_token)
         self.pos.fill_(m.length)
+        self.pos32.fill_(m.length)
         self.n_keys.fill_(m.length + 1)
         self.steps = 0
         if not self.graphs:

@@ -40,6 +40,9 @@ def parse_args(argv=None):
     ap.add_argument("--gamma", type=int, default=64)
     ap.add_argument("--gamma-dec", type=int, default=32)
     ap.add_argument("--layers", type=int, default=0, help="override the layer count (0 = the architecture's)")
+    ap.add_argument("--kv-cache", choices=["bf16", "e4m3", "int8"], default="bf16", help="format of the KV cache")
+    ap.add_argument("--kv-block", type=int, choices=[16, 32, 64, 128], default=64,
+                    help="tokens per scale of an 8-bit cache")
     ap.add_argument("--breakdown-steps", type=int, default=8)
     ap.add_argument("--eager-decode", action="store_true",
                     help="decode through the eager path (one launch sequence per layer from Python) "
@@ -77,7 +80,8 @@ def main(argv=None) -> int:
     if args.layers:
         arch = tiny(arch, n_layers=args.layers)
     cfg = Config(delta_lambda=args.gamma, sliding_window=args.window, sink=args.sink, mode="delta",
-                 decode_mode=args.decode_mode, gamma_dec=args.gamma_dec)
+                 decode_mode=args.decode_mode, gamma_dec=args.gamma_dec, kv_cache=args.kv_cache,
+                 kv_block=args.kv_block)
     model = DeltaDecoder(arch, cfg, TP(rank, world), device=dev, seed=0)
     g = torch.Generator(device=dev).manual_seed(1234)
     ids = torch.randint(0, arch.vocab, (args.batch, args.seq), generator=g, device=dev)
@@ -151,7 +155,7 @@ def main(argv=None) -> int:
                         f"TP over KV groups, delta prefill, {args.decode_mode} decode",
             "arch": arch.name, "n_layers": arch.n_layers, "n_gpus": world, "batch": args.batch,
             "prompt_tokens": args.seq, "new_tokens": args.new_tokens, "decode_mode": args.decode_mode,
-            "window": args.window, "sink": args.sink, "gamma": args.gamma,
+            "window": args.window, "sink": args.sink, "gamma": args.gamma, "kv_cache": args.kv_cache,
             "ttft_ms": ttft,
             "prefill_tokens_per_s": args.batch * args.seq / (ttft / 1e3),
             "decode_path": "eager" if args.eager_decode else "cuda graph per token",
