@@ -78,15 +78,15 @@ int sparse_chunk(long long sink, long long window) {
 // slots are shared with the sparse set in proportion to the keys, whether it is
 // wanted or not, so that a dense row is the same either way; the sparse chunks then
 // fill the slots that the dense ones leave.  Where sequences have lengths of their
-// own, about half of the chunks are taken to be empty.  `slots` 0: the shortest
-// chunk that any device gets.
+// own, about half of the chunks are taken to be empty.
 #ifndef DTA_CD_RAMP
 #define DTA_CD_RAMP 3
 #endif
 constexpr int kRampSteps = DTA_CD_RAMP, kWaves = 8;
+constexpr int kMaxSms = 160;  // SMs that are counted at most (a B200 has 148)
 
 int dense_chunk(long long n, long long sparse_keys, long long units, bool ragged, long long slots) {
-  if (slots <= 0 || n <= kChunkStep) return kChunkStep;
+  if (n <= kChunkStep) return kChunkStep;
   slots = slots * n / (n + sparse_keys);
   long long best = 0, best_cost = 0;
   for (int w = 1; w <= kWaves; ++w) {
@@ -105,6 +105,12 @@ int dense_chunk(long long n, long long sparse_keys, long long units, bool ragged
 
 // CTAs of the partial kernel that are resident on an SM (shared memory bounds them).
 int resident_ctas(int head_dim) { return head_dim == 128 ? 2 : 4; }
+
+// At most this many dense chunks per unit, on any device.
+long long dense_chunks_max(long long n, long long units, int head_dim) {
+  const long long k = (long long)kWaves * kMaxSms * resident_ctas(head_dim) / units, shortest = ceil_div(n, kChunkStep);
+  return k < 1 ? 1 : k < shortest ? k : shortest;
+}
 
 int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
   if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
@@ -127,7 +133,7 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   const long long sparse_keys = p->sink + (long long)p->window;
   const bool ragged = p->n_keys_dev && p->len_step;
   p->set[0].chunk = dense_chunk(n, sparse_keys < n ? sparse_keys : n, units, ragged,
-                                (long long)sms * resident_ctas(c.head_dim));
+                                (long long)(sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim));
   p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
   p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
   const int sc = sparse_chunk(p->sink, p->window);
@@ -139,8 +145,8 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   return DTA_OK;
 }
 
-size_t set_bytes(const dta_cache_decode_args* a, const dta::CacheDecodeSet& S) {
-  return align_up((size_t)a->cache.batch * a->n_heads * S.n_launched * (4 + a->cache.head_dim) * 4, 256);
+size_t partial_bytes(const dta_cache_decode_args* a, long long chunks) {
+  return align_up((size_t)a->cache.batch * a->n_heads * (chunks > 1 ? chunks : 1) * (4 + a->cache.head_dim) * 4, 256);
 }
 
 }  // namespace
@@ -203,17 +209,19 @@ int dta_cache_read(const dta_cache_read_args* a, void* stream) {
   return e == cudaSuccess ? (int)DTA_OK : dta::fail_cuda(e);
 }
 
-// Both key sets' partials, whichever outputs the call asks for, at the shortest
-// dense chunk (an upper bound for the chunk dta_cache_decode picks).
+// Both key sets' partials, whichever outputs the call asks for: enough for any
+// device, and never less for more keys (a caller may size it for the capacity once).
 size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
   dta::CacheDecodeParams p;
-  if (decode_setup(a, &p, 0) != DTA_OK) return 0;
-  return set_bytes(a, p.set[0]) + set_bytes(a, p.set[1]);
+  if (decode_setup(a, &p, 1) != DTA_OK) return 0;
+  const long long units = (long long)p.B * p.Hkv;
+  const int sparse = p.set[1].n_launched > kSparseTarget ? p.set[1].n_launched : kSparseTarget;
+  return partial_bytes(a, dense_chunks_max(a->n_keys, units, a->cache.head_dim)) + partial_bytes(a, sparse);
 }
 
 int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
   dta::CacheDecodeParams p;
-  int st = decode_setup(a, &p, 0);
+  int st = decode_setup(a, &p, 1);
   if (st != DTA_OK) return st;
   if (!a->q || (!a->dense_out && !a->sparse_out)) return DTA_ERR_INVALID_ARG;
   if (!aligned(a->q, 16) || !aligned(a->dense_out, 16) || !aligned(a->sparse_out, 16)) return DTA_ERR_ALIGNMENT;
@@ -226,7 +234,8 @@ int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
   p.q = reinterpret_cast<const __nv_bfloat16*>(a->q);
   p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
   p.set[0].partials = reinterpret_cast<float*>(a->workspace);
-  p.set[1].partials = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + set_bytes(a, p.set[0]));
+  p.set[1].partials = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) +
+                                                 partial_bytes(a, p.set[0].n_launched));
   p.out[0] = reinterpret_cast<__nv_bfloat16*>(a->dense_out);
   p.out[1] = reinterpret_cast<__nv_bfloat16*>(a->sparse_out);
   const cudaError_t e = dta::launch_cache_decode(p, a->cache.head_dim, a->cache.format, reinterpret_cast<cudaStream_t>(stream));

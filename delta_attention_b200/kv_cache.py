@@ -63,6 +63,7 @@ class QuantizedKV:
         self.batch, self.n_kv_heads, self.capacity, self.head_dim = b, Hkv, cap, d
         self.device = k.device
         self.index = k.device.index if k.device.type == "cuda" else None
+        self.workspace_bytes = {}  # of cache_decode, by (heads, window, sink)
         # the C ABI's argument structs with this cache filled in; each call copies one
         self._write_args, self._read_args, self._decode_args = CacheWriteArgs(), CacheReadArgs(), CacheDecodeArgs()
         for a in (self._write_args, self._read_args, self._decode_args):

@@ -326,7 +326,7 @@ def _decode_workspace(nbytes: int, device) -> torch.Tensor:
 
 
 def _stream_workspace(nbytes: int, index: int, stream: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return _workspace(nbytes, torch.device("cuda", index))
     key = (index, stream)
     ws = _decode_ws.get(key)
@@ -452,7 +452,7 @@ def _on_cache_device(op, cache, *args, **kw):
 
 
 def _is_current(cache: QuantizedKV) -> bool:
-    return cache.index is not None and cache.index == torch.cuda.current_device()
+    return cache.index is not None and cache.index == torch._C._cuda_getDevice()
 
 
 def _raw_stream(index: int) -> int:
@@ -566,6 +566,14 @@ def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int =
     return out
 
 
+def _cache_workspace_bytes(a: CacheDecodeArgs, cache: QuantizedKV) -> int:
+    """Workspace that serves every key count of this cache (it grows with the
+    count, so the capacity's is enough)."""
+    full = CacheDecodeArgs.from_buffer_copy(a)
+    full.n_keys = cache.capacity
+    return lib().dta_cache_decode_workspace_size(ctypes.byref(full))
+
+
 def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int, scaling: Optional[float] = None,
                  want_dense: bool = True, want_sparse: bool = True, n_keys: Optional[int] = None,
                  n_keys_dev: Optional[torch.Tensor] = None,
@@ -607,7 +615,10 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     if n_keys_dev is not None:
         a.n_keys_dev, a.n_lengths = _device_list(n_keys_dev, "n_keys_dev", cache), n_keys_dev.numel()
     L, stream = lib(), _raw_stream(cache.index)
-    ws = _stream_workspace(L.dta_cache_decode_workspace_size(ctypes.byref(a)), cache.index, stream)
+    size = cache.workspace_bytes.get((H, a.window, a.sink))
+    if size is None:
+        size = cache.workspace_bytes[(H, a.window, a.sink)] = _cache_workspace_bytes(a, cache)
+    ws = _stream_workspace(size, cache.index, stream)
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     _check_status(L.dta_cache_decode(ctypes.byref(a), stream), "dta_cache_decode")
     return dense, sparse

@@ -158,10 +158,18 @@ def test_abi_refuses_calls(kind, change, status):
 
 
 def test_decode_workspace_size():
+    """Never less for more keys, and bounded however long the cache is."""
     L = _lib.lib()
     a = _args(_lib.CacheDecodeArgs)
-    size = L.dta_cache_decode_workspace_size(ctypes.byref(a))
-    assert size > 0
+    a.cache.capacity = 1 << 30
+    for window, sink in ((64, 4), (0, 0), (1030, 128), (5000, 33), (1 << 30, 1 << 30)):
+        a.window, a.sink, last = window, sink, 0
+        for n in [*range(0, 3000, 37), 5000, 10000, 100000, 1 << 20, 1 << 25, 1 << 30]:
+            a.n_keys = n
+            size = L.dta_cache_decode_workspace_size(ctypes.byref(a))
+            assert size >= max(last, 1), (window, sink, n)
+            last = size
+        assert last <= 2 * 8 * (8 * 160 * 2 // 8 + 4200) * 132 * 4 + 512
     a.cache.block = 7
     assert L.dta_cache_decode_workspace_size(ctypes.byref(a)) == 0
 
