@@ -36,13 +36,28 @@ __device__ __forceinline__ int cache_need(float amax) {
   return max(u, 1);
 }
 
-// a * b elementwise (one instruction for two products).
-__device__ __forceinline__ float2 mul2(float2 a, float b) {
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
       "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
       : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b));
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// Two values -> two e4m3 codes, ties to even.
+__device__ __forceinline__ uint32_t e4m3_pack2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
 
@@ -51,12 +66,9 @@ __device__ __forceinline__ float2 mul2(float2 a, float b) {
 template <int FMT>
 __device__ __forceinline__ uint32_t cache_pack4(float2 a, float2 b, float inv) {
   if constexpr (FMT == CACHE_E4M3) {
-    a = mul2(a, inv);
-    b = mul2(b, inv);
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
-    return (uint32_t)lo | ((uint32_t)hi << 16);
+    a = mul2(a, make_float2(inv, inv));
+    b = mul2(b, make_float2(inv, inv));
+    return e4m3_pack2(a.x, a.y) | (e4m3_pack2(b.x, b.y) << 16);
   } else {
     // x * inv is exact, so x * inv + 1.5 * 2^23 rounds it once, to an integer in the low bits
     const float magic = 12582912.f;
@@ -66,34 +78,50 @@ __device__ __forceinline__ uint32_t cache_pack4(float2 a, float2 b, float inv) {
   }
 }
 
-// Two codes in the low (HI = 0) or high half of `w` -> two fp16 values (exact).
-template <int FMT, int HI>
-__device__ __forceinline__ uint32_t cache_half2(uint32_t w) {
+__device__ __forceinline__ uint32_t e4m3_half2(uint16_t h) {
   uint32_t r;
-  if constexpr (FMT == CACHE_E4M3) {
-    const uint16_t h = (uint16_t)(HI ? w >> 16 : w & 0xffffu);
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
-  } else {
-    // w holds code + 128 per byte: the byte under 0x64 is fp16 1024 + 128 + code
-    const uint32_t x = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
-  }
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(h));
   return r;
 }
-// What cache_half2 expects: e4m3 codes as they are, int8 codes with 128 added.
+// int8 codes in bytes 0 and 2 -> two fp16: the byte code + 128 under 0x64 is 1024 + 128 + code.
+__device__ __forceinline__ uint32_t int8_half2(uint32_t w) {
+  uint32_t r = (w & 0x00ff00ffu) ^ 0x64806480u;
+  asm("sub.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+  return r;
+}
+// Four codes of each of two rows -> four fp16 pairs (row a's code i, row b's code i), exact.
 template <int FMT>
-__device__ __forceinline__ uint32_t cache_bias(uint32_t w) {
-  return FMT == CACHE_INT8 ? w ^ 0x80808080u : w;
+__device__ __forceinline__ void cache_zip(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
+  if constexpr (FMT == CACHE_E4M3) {
+    const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
+    o[0] = e4m3_half2((uint16_t)(x & 0xffffu));
+    o[1] = e4m3_half2((uint16_t)(x >> 16));
+    o[2] = e4m3_half2((uint16_t)(y & 0xffffu));
+    o[3] = e4m3_half2((uint16_t)(y >> 16));
+  } else {
+    const uint32_t x = __byte_perm(a, b, 0x5410), y = __byte_perm(a, b, 0x7632);
+    o[0] = int8_half2(x);
+    o[1] = int8_half2(x >> 8);
+    o[2] = int8_half2(y);
+    o[3] = int8_half2(y >> 8);
+  }
 }
 
 // Four codes -> four fp32 values (unscaled).
 template <int FMT>
 __device__ __forceinline__ void cache_unpack4(uint32_t w, float (&f)[4]) {
-  const uint32_t b = cache_bias<FMT>(w);
-  const uint32_t lo = cache_half2<FMT, 0>(b), hi = cache_half2<FMT, 1>(b);
-  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+  if constexpr (FMT == CACHE_E4M3) {
+    const uint32_t lo = e4m3_half2((uint16_t)(w & 0xffffu)), hi = e4m3_half2((uint16_t)(w >> 16));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+  } else {
+    // code + 128 in the low byte under 2^23: an fp32 integer
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)) - (8388608.f + 128.f);
+  }
 }
 
 }  // namespace dta

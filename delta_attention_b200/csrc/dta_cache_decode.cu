@@ -7,9 +7,15 @@
 // l = sum 2^(s_j - m) and o = sum 2^(s_j + e_j - r) V_j (fp32); out = o 2^(r - m) / l.
 // The value scale enters the exponent, so the weights of o stay in (0, 1] whatever
 // the scales are, and are held in fp16 times 2^14 for the tensor cores (11 bits down
-// to 2^-28, more than bf16 has); codes convert to fp16 exactly.  Queries are scaled
-// per head by a power of two into fp16's range, which is exact down to 2^-29 of the
-// head's largest element.
+// to 2^-28, more than bf16 has); value codes are exact in fp16.
+//
+// The scores' operands.  e4m3: codes and queries in fp16, the queries scaled per head
+// by a power of two so that the largest element lies in [2^14, 2^15) (exact down to
+// 2^-29 of it); products and sums in fp32.  (The 8-bit mma.sync of this type converts
+// to fp16 itself: the kernel ran 25% more instructions with it.)  int8: codes as they
+// are, the query as a 16-bit integer, 32512 / max|q| times q (off by at most 2^-16 of
+// the largest element), in two 8-bit parts; products and sums in integers.  That costs no
+// conversion: 347 instructions for 16 keys, 364 to 398 with codes converted to fp16.
 //
 // Split-K over the cache: CTA (chunk, batch x KV head) reads its chunk's codes once
 // for all G <= 8 query heads of the group; the partials (m, l, r, o) of the chunks
@@ -49,6 +55,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_int8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Transposes an 8x8 matrix of 16-bit values held one row per lane quad.
@@ -156,9 +170,10 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
 // Partial kernel: CD_WARPS warps, each with a ring and a state of its own; warp w
 // takes the chunk's keys in steps of CD_KEYS, every CD_WARPS-th step.  With
 // (g, t) = (lane / 4, lane % 4) a step is, for each group of 16 keys,
-//   S^T (16 keys x 8 heads) = K Q^T   m16n8k16, A rows g and 8 + g = those keys;
-//                                     lane t holds pieces KP t + c of a row, and its
-//                                     word i of piece c feeds step (c, i)
+//   S^T (16 keys x 8 heads) = K Q^T   A rows g and 8 + g = those keys; lane t holds
+//                                     pieces KP t + c of a row; a word of four codes is a
+//                                     lane's part of one m16n8k16 step (e4m3), two words
+//                                     of one m16n8k32 step (int8)
 //   O^T (dims x 8 heads) += V^T P^T   lane (g, t) holds bytes [HD/8 g, HD/8 (g + 1)) of
 //                                     keys 2t, 2t+1, 2t+8, 2t+9: rows g and 8 + g of
 //                                     tile j are dims HD/8 g + 2j and + 1
@@ -253,7 +268,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // ---- Q as the B operand: head g, dims 16 (KP t + c) + 4 i + {0, 1} and + {2, 3} for step (c, i) ----
+  // ---- Q as the B operand: entry (c, i) holds head g's dims 16 (KP t + c) + 4 i + {0 .. 3}: as two
+  // fp16 pairs (e4m3), or their high and low bytes (int8) ----
   uint32_t qb[KP][4][2];
   float my_scale;
   {
@@ -274,17 +290,44 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       for (int e = 0; e < 8; ++e) top = max(top, max((w[c][e] << 16) & 0x7fffffffu, w[c][e] & 0x7fff0000u));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // bring the largest magnitude to [2^14, 2^15); a row with a non-finite element is NaN throughout
-    const int e = (int)(top >> 23);
-    const int up = e == 255 ? 0 : min(max(141 - e, -126), 126);
-    const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-    my_scale = e == 255 ? __uint_as_float(0x7fc00000u) : p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+    float f;
+    if constexpr (FMT == CACHE_E4M3) {
+      const int up = min(max(141 - (int)(top >> 23), -126), 126);
+      f = __uint_as_float((uint32_t)(127 + up) << 23);
+      my_scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+    } else {
+      const float most = fmaxf(__uint_as_float(top), 0x1p-100f);  // (a head that is all smaller counts as zeros)
+      f = 32512.f / most;
+      my_scale = p.scale_log2 * (most / 32512.f);
+    }
+    // a row with a non-finite element is NaN throughout
+    if (top >= 0x7f800000u) {
+      f = 0.f;
+      my_scale = __uint_as_float(0x7fc00000u);
+    }
 #pragma unroll
     for (int c = 0; c < KP; ++c)
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        qb[c][x >> 1][x & 1] =
-            pack_f16x2(__uint_as_float(w[c][x] << 16) * f, __uint_as_float(w[c][x] & 0xffff0000u) * f);
+      for (int i = 0; i < 4; ++i) {
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          d[2 * e] = __uint_as_float(w[c][2 * i + e] << 16) * f;
+          d[2 * e + 1] = __uint_as_float(w[c][2 * i + e] & 0xffff0000u) * f;
+        }
+        if constexpr (FMT == CACHE_E4M3) {
+          qb[c][i][0] = pack_f16x2(d[0], d[1]);
+          qb[c][i][1] = pack_f16x2(d[2], d[3]);
+        } else {
+          qb[c][i][0] = qb[c][i][1] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = __float2int_rn(d[e]), hi = (x + 128) >> 8;  // |x| <= 32512, so |hi| <= 127
+            qb[c][i][0] |= (uint32_t)(hi & 255) << (8 * e);
+            qb[c][i][1] |= (uint32_t)(x & 255) << (8 * e);  // x - 256 hi, in [-128, 127]
+          }
+        }
+      }
   }
   // score factors of this lane's columns, heads 2t and 2t + 1
   float sl[2];
@@ -331,18 +374,29 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     float s[NG][4];
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
+      int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
       s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KP; ++c) {
         uint32_t w0[4], w1[4];
         lds128(st + ka[c] + (q * CACHE_GROUP) * HD, w0);
         lds128(st + ka[c] + (q * CACHE_GROUP + 8) * HD, w1);
+        if constexpr (FMT == CACHE_E4M3) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = cache_bias<FMT>(w0[i]), y = cache_bias<FMT>(w1[i]);
-          mma_f16(s[q], cache_half2<FMT, 0>(x), cache_half2<FMT, 0>(y), cache_half2<FMT, 1>(x), cache_half2<FMT, 1>(y),
-                  qb[c][i][0], qb[c][i][1]);
+          for (int i = 0; i < 4; ++i)
+            mma_f16(s[q], e4m3_half2((uint16_t)(w0[i] & 0xffffu)), e4m3_half2((uint16_t)(w1[i] & 0xffffu)),
+                    e4m3_half2((uint16_t)(w0[i] >> 16)), e4m3_half2((uint16_t)(w1[i] >> 16)), qb[c][i][0], qb[c][i][1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            mma_int8(hi, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][0], qb[c][i + 1][0]);
+            mma_int8(lo, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][1], qb[c][i + 1][1]);
+          }
         }
+      }
+      if constexpr (FMT == CACHE_INT8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[q][e] = (float)(hi[e] * 256 + lo[e]);
       }
     }
     // ---- weights ----
@@ -351,10 +405,12 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     for (int q = 0; q < NG; ++q) {
       const float kf = cache_scale(ku[q]);
       ve[q] = vu[q] == 255 ? __uint_as_float(0x7fc00000u) : (float)(vu[q] - 127);
-      s[q][0] *= sl[0] * kf;
-      s[q][1] *= sl[1] * kf;
-      s[q][2] *= sl[0] * kf;
-      s[q][3] *= sl[1] * kf;
+      const float2 f = mul2(make_float2(sl[0], sl[1]), make_float2(kf, kf));
+      const float2 x = mul2(make_float2(s[q][0], s[q][1]), f), y = mul2(make_float2(s[q][2], s[q][3]), f);
+      s[q][0] = x.x;
+      s[q][1] = x.y;
+      s[q][2] = y.x;
+      s[q][3] = y.y;
     }
     if (base < k0 || base + CD_KEYS > k1) {
 #pragma unroll
@@ -398,17 +454,21 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
         }
       }
     }
-    const float mu[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-    const float ru[2] = {r[0] == -INFINITY ? 0.f : r[0], r[1] == -INFINITY ? 0.f : r[1]};
+    const float2 mu = make_float2(m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]);
+    const float2 ru = make_float2(r[0] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[0], r[1] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[1]);
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
+      const float2 off = add2(make_float2(ve[q], ve[q]), ru);
       float pw[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += fast_exp2(s[q][h] - mu[h]) + fast_exp2(s[q][2 + h] - mu[h]);
-        const float off = ve[q] - ru[h] + CD_SHIFT;
-        pw[h] = fast_exp2(s[q][h] + off);
-        pw[2 + h] = fast_exp2(s[q][2 + h] + off);
+      for (int e = 0; e < 2; ++e) {
+        const float2 x = make_float2(s[q][2 * e], s[q][2 * e + 1]);
+        const float2 a = add2(x, mu), c = add2(x, off);
+        const float2 w = add2(make_float2(l[0], l[1]), make_float2(fast_exp2(a.x), fast_exp2(a.y)));
+        l[0] = w.x;
+        l[1] = w.y;
+        pw[2 * e] = fast_exp2(c.x);
+        pw[2 * e + 1] = fast_exp2(c.y);
       }
       const uint32_t b0 = movmatrix_t(pack_f16x2(pw[0], pw[1]));
       const uint32_t b1 = movmatrix_t(pack_f16x2(pw[2], pw[3]));
@@ -422,14 +482,11 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       }
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
-        const uint32_t wa = cache_bias<FMT>(v[0][i]), wb = cache_bias<FMT>(v[1][i]);
-        const uint32_t wc = cache_bias<FMT>(v[2][i]), wd = cache_bias<FMT>(v[3][i]);
-        const uint32_t ab = __byte_perm(wa, wb, 0x5140), AB = __byte_perm(wa, wb, 0x7362);
-        const uint32_t cd = __byte_perm(wc, wd, 0x5140), CD = __byte_perm(wc, wd, 0x7362);
-        mma_f16(o[2 * i], cache_half2<FMT, 0>(ab), cache_half2<FMT, 1>(ab), cache_half2<FMT, 0>(cd),
-                cache_half2<FMT, 1>(cd), b0, b1);
-        mma_f16(o[2 * i + 1], cache_half2<FMT, 0>(AB), cache_half2<FMT, 1>(AB), cache_half2<FMT, 0>(CD),
-                cache_half2<FMT, 1>(CD), b0, b1);
+        uint32_t ab[4], cd[4];
+        cache_zip<FMT>(v[0][i], v[1][i], ab);
+        cache_zip<FMT>(v[2][i], v[3][i], cd);
+        mma_f16(o[2 * i], ab[0], ab[1], cd[0], cd[1], b0, b1);
+        mma_f16(o[2 * i + 1], ab[2], ab[3], cd[2], cd[3], b0, b1);
       }
     }
     __syncwarp();  // the slot may be refilled

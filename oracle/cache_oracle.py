@@ -70,10 +70,11 @@ def key_set(n: int, window: int, sink: int, sparse: bool) -> torch.Tensor:
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n: int, scaling: float, window: int, sink: int,
-           sparse: bool):
-    """One sequence: q [H, d], k and v [Hkv, cap, d] values.  Returns (out,
-    spread, slack) [H, d]: the attention, the same weights over |v|, and the
-    part of the tolerance that comes from rounding the scores."""
+           sparse: bool, sum_step: float = 0.0, query_step: float = 0.0):
+    """One sequence: q [H, d], k and v [Hkv, cap, d] values.  Returns (out, spread,
+    slack) [H, d]: the attention, the same weights over |v|, and what scores that are
+    off by ``sum_step`` of |q| . |k| plus ``query_step`` of max|q| sum|k| (times the
+    scaling) can move the attention by, to first order."""
     H, d = q.shape
     G = H // k.shape[0]
     keys = key_set(n, window, sink, sparse)
@@ -85,6 +86,6 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n: int, scaling: f
         w = torch.softmax(kk @ qq * scaling, dim=0)
         out[h] = w @ vv
         spread[h] = w @ vv.abs()
-        mags = (kk.abs() @ qq.abs()) * scaling  # |q| . |k|: bounds the fp32 sums and the score itself
-        slack[h] = (w * mags) @ vv.abs() + (w @ mags) * spread[h]
+        off = (sum_step * (kk.abs() @ qq.abs()) + query_step * qq.abs().max() * kk.abs().sum(dim=1)) * scaling
+        slack[h] = (w * off) @ vv.abs() + (w @ off) * spread[h]
     return out, spread, slack

@@ -5,14 +5,14 @@ Writing and reading are exact: scales are powers of two, so a code is one
 rounding of an exact product and must equal the oracle's, bit for bit.
 
 Attention is held to, per output element with weights w, W = sum w |v| and
-M_j = scaling * |q| . |k_j|:
+off_j = scaling * (c |q| . |k_j| + e max|q| sum|k_j|):
   2^-8 |out|             the output's rounding to bf16 (half a step)
   2^-11 W                the weights' rounding to fp16
   n 2^-38 max|v|         weights below fp16's normal range (half a step is 2^-25 of 2^14, over l >= 1)
-  c (sum w M |v| + (sum w M) W)   the scores: q . k summed in fp32 over d terms, each partial sum off
-                         by at most 2^-23 of |q| . |k| (d steps, and 6 more for the products with the
-                         scales and log2 e), which moves a weight and the sum of the weights relatively
-                         by as much: c = (d + 6) 2^-23
+  sum w off |v| + (sum w off) W   the scores, off by off_j, move a weight and the sum of the weights
+                         relatively by as much.  c = (d + 6) 2^-23: sums over d terms in fp32 (d steps,
+                         and 6 more for the products with the scales and log2 e).  e: the query's own
+                         rounding, 2^-29 for e4m3 (fp16, scaled) and 2^-16 for int8 (16 bits)
   2^-13 W                sums of weights and products in fp32 (at most 2^9 steps of 2^-23 each in a warp's
                          share, and the merges), exp2's 2^-22, the maxima's shifts
 """
@@ -228,10 +228,10 @@ def _check_rows(got, q, cache, n, window, sink, sparse, what, scaling=None):
     scaling = d ** -0.5 if scaling is None else scaling
     kv = [orc.values(c, s, cache.block) for c, s in _state(cache)]
     for i in range(cache.batch):
-        out, spread, slack = orc.attend(q[i, :, 0].float().cpu(), kv[0][i], kv[1][i], n[i], scaling, window, sink, sparse)
+        out, spread, slack = orc.attend(q[i, :, 0].float().cpu(), kv[0][i], kv[1][i], n[i], scaling, window, sink,
+                                        sparse, (d + 6) * 2.0 ** -23, 2.0 ** (-16 if cache.format == "int8" else -29))
         vmax = kv[1][i, :, :n[i]].abs().amax().item() if n[i] else 0.0
-        tol = 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + n[i] * 2.0 ** -38 * vmax \
-            + (d + 6) * 2.0 ** -23 * slack
+        tol = 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + n[i] * 2.0 ** -38 * vmax + slack
         err = (got[i, 0].float().cpu().double() - out).abs()
         assert torch.isfinite(got[i].float()).all(), f"{what}: sequence {i} not finite"
         worst = (err / tol.clamp_min(1e-300)).max().item() if n[i] else float(err.max() > 0)
