@@ -47,6 +47,9 @@ struct CacheReadParams {
 // block; only a key set's own first and last key may lie inside a group.
 constexpr int CACHE_GROUP = 16;
 
+// Keys in one step of a CTA of the decode kernel, and what its start and end cost, in steps.
+constexpr int CACHE_STEP = 128, CACHE_RAMP_STEPS = 3;
+
 struct CacheDecodeSet {
   int chunk;               // keys per chunk, a multiple of CACHE_GROUP
   int n_sink_chunks;       // sparse set: chunks that cover [0, sink)
@@ -64,6 +67,7 @@ struct CacheDecodeParams {
   float scale_log2;
   int window, sink;
   int clusters;            // whether chunks may merge within a cluster
+  int slots;               // CTAs of the decode kernel that are resident at once
   CacheDecodeSet set[2];   // 0: dense, 1: sparse
   __nv_bfloat16* out[2];   // dense, sparse; either may be null
 };

@@ -59,7 +59,7 @@ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 #ifndef DTA_CD_SPARSE_TARGET
 #define DTA_CD_SPARSE_TARGET 9
 #endif
-constexpr int kChunkStep = 128;  // one step of a CTA's warps
+constexpr int kChunkStep = dta::CACHE_STEP;  // one step of a CTA's warps
 constexpr int kSparseTarget = DTA_CD_SPARSE_TARGET, kSparseChunkMax = 512, kSparseChunk = 256,
               kSparseChunks = 2048;
 
@@ -71,33 +71,36 @@ int sparse_chunk(long long sink, long long window) {
   return (int)(c > kSparseChunk ? c : kSparseChunk);
 }
 
-// Chunk of the dense set: the one with the least estimated time.  With `slots` CTAs
-// resident at once, w waves of them take k = w slots / units chunks of each unit (a
-// (batch, KV head)), and cost w times a chunk's steps plus kRampSteps for a CTA's
-// start and end (a step takes 1.5 us while the memory is saturated).  The
-// slots are shared with the sparse set in proportion to the keys, whether it is
-// wanted or not, so that a dense row is the same either way; the sparse chunks then
-// fill the slots that the dense ones leave.  Where sequences have lengths of their
-// own, about half of the chunks are taken to be empty.
-#ifndef DTA_CD_RAMP
-#define DTA_CD_RAMP 3
-#endif
-constexpr int kRampSteps = DTA_CD_RAMP, kWaves = 8;
+// Chunk of the dense set: the one with the least estimated time, in steps of a CTA.
+// With `slots` CTAs resident at once, w waves of them take k = w slots / units chunks
+// of each unit (a (batch, KV head)); a CTA costs its chunk's steps plus kRampSteps
+// for its start and end (a step takes 1.5 us while the memory is saturated).  The
+// sparse set's CTAs, if they are wanted too, come last: into the places that the
+// dense ones leave, else after them, so fewer chunks that leave them room are tried as
+// well.  Where sequences have lengths of their own, about half of the chunks are taken
+// to be empty.  (16 sequences of 8191 down to 0 keys, 8 KV heads: 29.6 us with 2048-key
+// chunks, 32.6 with 1024, 38.3 with 4096.  32761 keys, 8 KV heads of 8 queries, both
+// rows: 21.8 us with 1280, which leaves the sparse chunks room, 25.1 with 896.)
+constexpr int kRampSteps = dta::CACHE_RAMP_STEPS, kWaves = 8;
 constexpr int kMaxSms = 160;  // SMs that are counted at most (a B200 has 148)
 
-int dense_chunk(long long n, long long sparse_keys, long long units, bool ragged, long long slots) {
+int dense_chunk(long long n, long long units, long long sparse_ctas, long long sparse_steps, bool ragged,
+                long long slots) {
   if (n <= kChunkStep) return kChunkStep;
-  slots = slots * n / (n + sparse_keys);
+  const long long sparse_cost = sparse_steps + kRampSteps;
   long long best = 0, best_cost = 0;
-  for (int w = 1; w <= kWaves; ++w) {
-    const long long k = w * slots / units > 0 ? w * slots / units : 1;
-    const long long steps = ceil_div(n, k * kChunkStep);
-    const long long chunks = ceil_div(n, steps * kChunkStep) * units;
-    const long long waves = ragged ? ceil_div(chunks, 2 * slots) : ceil_div(chunks, slots);
-    const long long cost = waves * (steps + kRampSteps);
-    if (best == 0 || cost < best_cost) {
+  for (int i = 0; i < 2 * kWaves; ++i) {
+    const long long room = i & 1 ? (sparse_ctas < slots / 2 ? sparse_ctas : slots / 2) : 0;
+    const long long places = (i / 2 + 1) * slots - room, k = places / units > 0 ? places / units : 1;
+    const long long steps = ceil_div(n, k * kChunkStep), cost = steps + kRampSteps;
+    const long long ctas = ceil_div(ceil_div(n, steps * kChunkStep) * units, ragged ? 2 : 1);
+    const long long waves = ceil_div(ctas, slots);
+    const long long beside = (waves * slots - ctas) * (cost / sparse_cost);
+    const long long after = sparse_ctas > beside ? ceil_div(sparse_ctas - beside, slots) * sparse_cost : 0;
+    const long long total = waves * cost + after;
+    if (best == 0 || total < best_cost) {
       best = steps * kChunkStep;
-      best_cost = cost;
+      best_cost = total;
     }
   }
   return (int)best;
@@ -130,16 +133,16 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   p->window = a->window < a->n_keys ? a->window : a->n_keys;
   p->sink = a->sink < a->n_keys ? a->sink : a->n_keys;
   const long long units = (long long)c.batch * c.n_kv_heads, n = a->n_keys;
-  const long long sparse_keys = p->sink + (long long)p->window;
-  const bool ragged = p->n_keys_dev && p->len_step;
-  p->set[0].chunk = dense_chunk(n, sparse_keys < n ? sparse_keys : n, units, ragged,
-                                (long long)(sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim));
-  p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
-  p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
   const int sc = sparse_chunk(p->sink, p->window);
   p->set[1].chunk = sc;
   p->set[1].n_sink_chunks = (int)ceil_div(p->sink, sc);
   p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, sc);
+  const bool ragged = p->n_keys_dev && p->len_step;
+  p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
+  p->slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim);
+  p->set[0].chunk = dense_chunk(n, units, a->sparse_out ? units * p->set[1].n_launched : 0, sc / kChunkStep, ragged,
+                                p->slots);
+  p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
   for (dta::CacheDecodeSet& S : p->set)
     if (S.n_launched < 1) S.n_launched = 1;  // no keys: one empty partial
   return DTA_OK;

@@ -47,6 +47,7 @@ constexpr int CD_WARPS = DTA_CD_WARPS;
 constexpr int CD_THREADS = CD_WARPS * 32;
 constexpr int CD_KEYS = DTA_CD_KEYS;      // keys per step of a warp
 constexpr int CD_STAGES = DTA_CD_STAGES;  // steps in flight per warp
+static_assert(CD_WARPS * CD_KEYS == CACHE_STEP, "the host counts the same steps");
 constexpr float CD_SHIFT = 14.f;  // log2 of the factor that the fp16 weights carry
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -636,12 +637,12 @@ __global__ void __launch_bounds__(MG_ROWS* HD) cache_merge_kernel(const __grid_c
 }
 
 // Sets the kernel's launch attributes on the current device, once per device (they
-// stay set), and for a cluster size asks whether such a cluster can be scheduled.
+// stay set); for a cluster size, *active is how many such clusters are resident at once.
 template <int HD, int FMT, bool CLU>
-static cudaError_t prepare_kernel(int nct, bool* fits) {
+static cudaError_t prepare_kernel(int nct, int* active) {
   constexpr int kDevices = 64;
   static std::mutex mu;
-  static std::atomic<int> state[kDevices][CD_CLUSTER_MAX + 1];  // 0 unknown, 1 ready, 2 does not fit
+  static std::atomic<int> state[kDevices][CD_CLUSTER_MAX + 1];  // 0 unknown, else 1 + clusters
   auto kernel = cache_decode_kernel<HD, FMT, CLU>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -670,9 +671,9 @@ static cudaError_t prepare_kernel(int nct, bool* fits) {
         n = 0;
       }
     }
-    st.store(n > 0 ? 1 : 2, std::memory_order_release);
+    st.store(1 + n, std::memory_order_release);
   }
-  *fits = st.load(std::memory_order_acquire) == 1;
+  *active = st.load(std::memory_order_acquire) - 1;
   return cudaSuccess;
 }
 
@@ -699,13 +700,20 @@ static cudaError_t decode_as(const CacheDecodeParams& p, cudaStream_t stream) {
   int nct = 0;
   for (int which = 0; which < 2; ++which)
     if (p.out[which]) nct += p.set[which].n_launched;
-  bool fits = false;
+  int active = 0;
   cudaError_t e;
   if (p.clusters && nct <= CD_CLUSTER_MAX) {
-    if ((e = prepare_kernel<HD, FMT, true>(nct, &fits)) != cudaSuccess) return e;
-    if (fits) return launch_partials<HD, FMT, true>(p, nct, stream);
+    // A cluster's CTAs lie in one GPC, so fewer CTAs are resident as clusters than
+    // alone (32 clusters of 9 take two waves where 288 CTAs take one: 123 us for
+    // 83 at 4 x 65536 keys); against that stands the merge launch, about two steps.
+    if ((e = prepare_kernel<HD, FMT, true>(nct, &active)) != cudaSuccess) return e;
+    const long long units = (long long)p.B * p.Hkv;
+    const int chunk = p.out[0] && p.set[0].chunk > p.set[1].chunk ? p.set[0].chunk : p.set[1].chunk;
+    const long long cost = chunk / CACHE_STEP + CACHE_RAMP_STEPS;
+    if (active > 0 && (units + active - 1) / active * cost <= (units * nct + p.slots - 1) / p.slots * cost + 2)
+      return launch_partials<HD, FMT, true>(p, nct, stream);
   }
-  if ((e = prepare_kernel<HD, FMT, false>(0, &fits)) != cudaSuccess) return e;
+  if ((e = prepare_kernel<HD, FMT, false>(0, &active)) != cudaSuccess) return e;
   if ((e = launch_partials<HD, FMT, false>(p, nct, stream)) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.B * p.H, (p.out[0] ? 1 : 0) + (p.out[1] ? 1 : 0));

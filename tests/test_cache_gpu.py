@@ -261,8 +261,10 @@ def test_decode(fmt, b, H, Hkv, d, block, cap, n, window, sink):
     dense, sparse = ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live)
     _check_rows(dense, q, cache, n, window, sink, False, "dense")
     _check_rows(sparse, q, cache, n, window, sink, True, "sparse")
-    # one row alone is the same row
-    assert torch.equal(ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_sparse=False)[0], dense)
+    # one row alone: the sparse row is the same bit for bit (its chunks go by sink and window only)
+    alone, none = ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_sparse=False)
+    assert none is None
+    _check_rows(alone, q, cache, n, window, sink, False, "dense alone")
     assert torch.equal(ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_dense=False)[1], sparse)
     if len(set(n)) == 1:  # a host count
         dense, sparse = ops.cache_decode(q, cache, window=window, sink=sink, n_keys=n[0])
