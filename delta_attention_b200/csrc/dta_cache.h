@@ -67,7 +67,6 @@ struct CacheDecodeParams {
   float scale_log2;
   int window, sink;
   int clusters;            // whether chunks may merge within a cluster
-  int slots;               // CTAs of the decode kernel that are resident at once
   CacheDecodeSet set[2];   // 0: dense, 1: sparse
   __nv_bfloat16* out[2];   // dense, sparse; either may be null
 };

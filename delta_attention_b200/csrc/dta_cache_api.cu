@@ -52,23 +52,46 @@ int check_list(const int32_t* list, int n, int batch, int* step) {
 
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Chunk of the sparse set: the shortest multiple of kChunkStep whose sink and window
-// chunks number at most kSparseTarget, up to kSparseChunkMax (they then merge within a
-// cluster: one launch for a sparse-only step); beyond, kSparseChunk.  A function of
-// (sink, window) only, so that a sparse row is the same whichever call it comes from.
-#ifndef DTA_CD_SPARSE_TARGET
-#define DTA_CD_SPARSE_TARGET 9
-#endif
 constexpr int kChunkStep = dta::CACHE_STEP;  // one step of a CTA's warps
-constexpr int kSparseTarget = DTA_CD_SPARSE_TARGET, kSparseChunkMax = 512, kSparseChunk = 256,
-              kSparseChunks = 2048;
+constexpr int kRampSteps = dta::CACHE_RAMP_STEPS;
+constexpr int kMaxSms = 160;  // SMs that are counted at most (a B200 has 148)
 
-int sparse_chunk(long long sink, long long window) {
-  for (int c = kChunkStep; c <= kSparseChunkMax; c += kChunkStep)
-    if (ceil_div(sink, c) + ceil_div(window, c) <= kSparseTarget) return c;
-  // (a launch has at most 65535 chunks: a window of millions of keys gets longer ones)
-  const long long c = ceil_div(ceil_div(sink + window, kSparseChunks), kChunkStep) * kChunkStep;
-  return (int)(c > kSparseChunk ? c : kSparseChunk);
+// CTAs of the partial kernel that are resident on an SM (shared memory bounds them).
+int resident_ctas(int head_dim) { return head_dim == 128 ? 2 : 4; }
+
+// Chunk of the sparse set, by the estimated time of its CTAs in steps: one that all are
+// resident with costs its own steps and kRampSteps; more of them the sum of their
+// costs over the slots and half a chunk's for the end; beyond 16 chunks per unit a
+// merge launch, two steps.  (128 + 2048 keys, 8 units: 6.0 us with 256-key chunks, 6.4 with
+// 384.)  It goes by sink, window, batch and heads only, so that a sparse row of a cache
+// is the same whichever call it comes from.
+constexpr int kSparseSteps[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
+constexpr int kSparseWaves = 4;  // chunks that would take more waves are not tried
+constexpr long long kSparseKeys = 1 << 23;  // windows beyond this take longer chunks (a launch has 65535 at most)
+
+int sparse_chunk(long long sink, long long window, long long units, long long slots) {
+  const long long f = sink + window > kSparseKeys ? ceil_div(sink + window, kSparseKeys) : 1;
+  const long long longest = f * kSparseSteps[sizeof(kSparseSteps) / sizeof(int) - 1];
+  long long best = longest, best_cost = -1;
+  for (int st : kSparseSteps) {
+    const long long steps = f * st, c = steps * kChunkStep, k = ceil_div(sink, c) + ceil_div(window, c);
+    if (units * k > kSparseWaves * slots && steps != longest) continue;
+    const long long sum = ceil_div(sink, kChunkStep) + ceil_div(window, kChunkStep) + k * kRampSteps;
+    const long long cost = (units * k <= slots ? 2 * (steps + kRampSteps) : 2 * units * sum / slots + steps + kRampSteps) +
+                           (k > 16 ? 4 : 0);
+    if (best_cost < 0 || cost < best_cost) {
+      best = steps;
+      best_cost = cost;
+    }
+  }
+  return (int)best * kChunkStep;
+}
+// At most this many sparse chunks of all units, on any device and for any smaller sink and window.
+long long sparse_chunks_max(long long sink, long long window, long long units, int head_dim) {
+  const long long few = (long long)kSparseWaves * kMaxSms * resident_ctas(head_dim);
+  const long long chunks = ceil_div(sink + window, 32 * kChunkStep), most = kSparseKeys / (32 * kChunkStep);
+  const long long many = units * ((chunks < most ? chunks : most) + 2);
+  return few > many ? few : many;
 }
 
 // Chunk of the dense set: the one with the least estimated time, in steps of a CTA.
@@ -80,18 +103,18 @@ int sparse_chunk(long long sink, long long window) {
 // well.  Where sequences have lengths of their own, about half of the chunks are taken
 // to be empty.  (16 sequences of 8191 down to 0 keys, 8 KV heads: 29.6 us with 2048-key
 // chunks, 32.6 with 1024, 38.3 with 4096.  32761 keys, 8 KV heads of 8 queries, both
-// rows: 21.8 us with 1280, which leaves the sparse chunks room, 25.1 with 896.)
-constexpr int kRampSteps = dta::CACHE_RAMP_STEPS, kWaves = 8;
-constexpr int kMaxSms = 160;  // SMs that are counted at most (a B200 has 148)
+// rows: 21.5 us with 1152, which leaves the sparse chunks room, 25.1 with 896.)
+constexpr int kWaves = 8;
 
 int dense_chunk(long long n, long long units, long long sparse_ctas, long long sparse_steps, bool ragged,
                 long long slots) {
   if (n <= kChunkStep) return kChunkStep;
   const long long sparse_cost = sparse_steps + kRampSteps;
   long long best = 0, best_cost = 0;
-  for (int i = 0; i < 2 * kWaves; ++i) {
-    const long long room = i & 1 ? (sparse_ctas < slots / 2 ? sparse_ctas : slots / 2) : 0;
-    const long long places = (i / 2 + 1) * slots - room, k = places / units > 0 ? places / units : 1;
+  for (int i = 0; i < 3 * kWaves; ++i) {
+    if (sparse_ctas == 0 && i % 3 != 0) continue;
+    const long long room = i % 3 * (sparse_ctas < slots / 2 ? sparse_ctas : slots / 2) / 2;
+    const long long places = (i / 3 + 1) * slots - room, k = places / units > 0 ? places / units : 1;
     const long long steps = ceil_div(n, k * kChunkStep), cost = steps + kRampSteps;
     const long long ctas = ceil_div(ceil_div(n, steps * kChunkStep) * units, ragged ? 2 : 1);
     const long long waves = ceil_div(ctas, slots);
@@ -105,9 +128,6 @@ int dense_chunk(long long n, long long units, long long sparse_ctas, long long s
   }
   return (int)best;
 }
-
-// CTAs of the partial kernel that are resident on an SM (shared memory bounds them).
-int resident_ctas(int head_dim) { return head_dim == 128 ? 2 : 4; }
 
 // At most this many dense chunks per unit, on any device.
 long long dense_chunks_max(long long n, long long units, int head_dim) {
@@ -133,23 +153,24 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   p->window = a->window < a->n_keys ? a->window : a->n_keys;
   p->sink = a->sink < a->n_keys ? a->sink : a->n_keys;
   const long long units = (long long)c.batch * c.n_kv_heads, n = a->n_keys;
-  const int sc = sparse_chunk(p->sink, p->window);
+  const long long slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim);
+  const int sc = sparse_chunk(p->sink, p->window, units, slots);
   p->set[1].chunk = sc;
   p->set[1].n_sink_chunks = (int)ceil_div(p->sink, sc);
   p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, sc);
   const bool ragged = p->n_keys_dev && p->len_step;
   p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
-  p->slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim);
   p->set[0].chunk = dense_chunk(n, units, a->sparse_out ? units * p->set[1].n_launched : 0, sc / kChunkStep, ragged,
-                                p->slots);
+                                slots);
   p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
   for (dta::CacheDecodeSet& S : p->set)
     if (S.n_launched < 1) S.n_launched = 1;  // no keys: one empty partial
   return DTA_OK;
 }
 
+// Bytes of the partials of `chunks` chunks (of all units together), each of a unit's query heads.
 size_t partial_bytes(const dta_cache_decode_args* a, long long chunks) {
-  return align_up((size_t)a->cache.batch * a->n_heads * (chunks > 1 ? chunks : 1) * (4 + a->cache.head_dim) * 4, 256);
+  return align_up((size_t)chunks * (a->n_heads / a->cache.n_kv_heads) * (4 + a->cache.head_dim) * 4, 256);
 }
 
 }  // namespace
@@ -218,8 +239,8 @@ size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
   dta::CacheDecodeParams p;
   if (decode_setup(a, &p, 1) != DTA_OK) return 0;
   const long long units = (long long)p.B * p.Hkv;
-  const int sparse = p.set[1].n_launched > kSparseTarget ? p.set[1].n_launched : kSparseTarget;
-  return partial_bytes(a, dense_chunks_max(a->n_keys, units, a->cache.head_dim)) + partial_bytes(a, sparse);
+  return partial_bytes(a, units * dense_chunks_max(a->n_keys, units, a->cache.head_dim)) +
+         partial_bytes(a, sparse_chunks_max(p.sink, p.window, units, a->cache.head_dim));
 }
 
 int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
@@ -238,7 +259,7 @@ int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
   p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
   p.set[0].partials = reinterpret_cast<float*>(a->workspace);
   p.set[1].partials = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) +
-                                                 partial_bytes(a, p.set[0].n_launched));
+                                                 partial_bytes(a, (long long)p.B * p.Hkv * p.set[0].n_launched));
   p.out[0] = reinterpret_cast<__nv_bfloat16*>(a->dense_out);
   p.out[1] = reinterpret_cast<__nv_bfloat16*>(a->sparse_out);
   const cudaError_t e = dta::launch_cache_decode(p, a->cache.head_dim, a->cache.format, reinterpret_cast<cudaStream_t>(stream));

@@ -703,15 +703,12 @@ static cudaError_t decode_as(const CacheDecodeParams& p, cudaStream_t stream) {
   int active = 0;
   cudaError_t e;
   if (p.clusters && nct <= CD_CLUSTER_MAX) {
-    // A cluster's CTAs lie in one GPC, so fewer CTAs are resident as clusters than
-    // alone (32 clusters of 9 take two waves where 288 CTAs take one: 123 us for
-    // 83 at 4 x 65536 keys); against that stands the merge launch, about two steps.
+    // Clusters save the merge launch (2.5 us of host time, 0.3 us of the GPU's) where
+    // they are all resident at once.  A cluster's CTAs lie in one GPC, so fewer are than
+    // of single CTAs, and a second wave costs more than the launch: 123 us for 83 with
+    // 32 clusters of 9 at 4 x 65536 keys.
     if ((e = prepare_kernel<HD, FMT, true>(nct, &active)) != cudaSuccess) return e;
-    const long long units = (long long)p.B * p.Hkv;
-    const int chunk = p.out[0] && p.set[0].chunk > p.set[1].chunk ? p.set[0].chunk : p.set[1].chunk;
-    const long long cost = chunk / CACHE_STEP + CACHE_RAMP_STEPS;
-    if (active > 0 && (units + active - 1) / active * cost <= (units * nct + p.slots - 1) / p.slots * cost + 2)
-      return launch_partials<HD, FMT, true>(p, nct, stream);
+    if ((long long)p.B * p.Hkv <= active) return launch_partials<HD, FMT, true>(p, nct, stream);
   }
   if ((e = prepare_kernel<HD, FMT, false>(0, &active)) != cudaSuccess) return e;
   if ((e = launch_partials<HD, FMT, false>(p, nct, stream)) != cudaSuccess) return e;

@@ -169,7 +169,7 @@ def test_decode_workspace_size():
             size = L.dta_cache_decode_workspace_size(ctypes.byref(a))
             assert size >= max(last, 1), (window, sink, n)
             last = size
-        assert last <= 2 * 8 * (8 * 160 * 2 // 8 + 4200) * 132 * 4 + 512
+        assert last <= (8 * 160 * 2 + 8 * 2050) * 2 * 132 * 4 + 512
     a.cache.block = 7
     assert L.dta_cache_decode_workspace_size(ctypes.byref(a)) == 0
 
