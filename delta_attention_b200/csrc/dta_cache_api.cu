@@ -95,7 +95,11 @@ long long sparse_chunks_max(long long sink, long long window, long long units, i
 }
 
 // Chunk of the dense set: the one with the least estimated time, in steps of a CTA.
-// With `slots` CTAs resident at once, w waves of them take k = w slots / units chunks
+// 7/8 of the resident CTAs are used (the sparse ones take the rest where they are
+// wanted): the memory is saturated by them, and SMs that have one CTA instead of two
+// even out at the end (131072 keys, 8 KV heads: 47.1 us
+// with 256 CTAs, 48.6 with 296, 55 with 168; 4 x 65536: 82.1 with 256, 88.8 with 288,
+// 92 with 192).  With that many `slots`, w waves of them take k = w slots / units chunks
 // of each unit (a (batch, KV head)); a CTA costs its chunk's steps plus kRampSteps
 // for its start and end (a step takes 1.5 us while the memory is saturated).  The
 // sparse set's CTAs, if they are wanted too, come last: into the places that the
@@ -104,11 +108,12 @@ long long sparse_chunks_max(long long sink, long long window, long long units, i
 // to be empty.  (16 sequences of 8191 down to 0 keys, 8 KV heads: 29.6 us with 2048-key
 // chunks, 32.6 with 1024, 38.3 with 4096.  32761 keys, 8 KV heads of 8 queries, both
 // rows: 21.5 us with 1152, which leaves the sparse chunks room, 25.1 with 896.)
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 
 int dense_chunk(long long n, long long units, long long sparse_ctas, long long sparse_steps, bool ragged,
                 long long slots) {
   if (n <= kChunkStep) return kChunkStep;
+  if (sparse_ctas == 0 && slots > 1) slots = slots * 7 / 8;
   const long long sparse_cost = sparse_steps + kRampSteps;
   long long best = 0, best_cost = 0;
   for (int i = 0; i < 3 * kWaves; ++i) {
@@ -135,7 +140,8 @@ long long dense_chunks_max(long long n, long long units, int head_dim) {
   return k < 1 ? 1 : k < shortest ? k : shortest;
 }
 
-int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
+// Checks the arguments (no CUDA call) and fills in all but the plan.
+int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p) {
   if (!a || a->abi_version != DTA_ABI_VERSION) return DTA_ERR_INVALID_ARG;
   memset(p, 0, sizeof(*p));
   const dta_cache_desc& c = a->cache;
@@ -152,20 +158,27 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int 
   // sink and window beyond the cache mean the whole cache
   p->window = a->window < a->n_keys ? a->window : a->n_keys;
   p->sink = a->sink < a->n_keys ? a->sink : a->n_keys;
-  const long long units = (long long)c.batch * c.n_kv_heads, n = a->n_keys;
-  const long long slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(c.head_dim);
-  const int sc = sparse_chunk(p->sink, p->window, units, slots);
-  p->set[1].chunk = sc;
-  p->set[1].n_sink_chunks = (int)ceil_div(p->sink, sc);
-  p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, sc);
+  return DTA_OK;
+}
+
+// The chunks of the sets that are wanted, for a device of `sms` SMs.
+void decode_plan(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
+  const long long units = (long long)p->B * p->Hkv, n = p->n_keys;
+  const long long slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(a->cache.head_dim);
   const bool ragged = p->n_keys_dev && p->len_step;
   p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
-  p->set[0].chunk = dense_chunk(n, units, a->sparse_out ? units * p->set[1].n_launched : 0, sc / kChunkStep, ragged,
-                                slots);
-  p->set[0].n_launched = (int)ceil_div(n, p->set[0].chunk);
-  for (dta::CacheDecodeSet& S : p->set)
-    if (S.n_launched < 1) S.n_launched = 1;  // no keys: one empty partial
-  return DTA_OK;
+  if (a->sparse_out) {
+    const int c = sparse_chunk(p->sink, p->window, units, slots);
+    p->set[1].chunk = c;
+    p->set[1].n_sink_chunks = (int)ceil_div(p->sink, c);
+    p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, c);
+    if (p->set[1].n_launched < 1) p->set[1].n_launched = 1;  // no keys: one empty partial
+  }
+  if (a->dense_out) {
+    const int c = dense_chunk(n, units, units * p->set[1].n_launched, p->set[1].chunk / kChunkStep, ragged, slots);
+    p->set[0].chunk = c;
+    p->set[0].n_launched = n > 0 ? (int)ceil_div(n, c) : 1;
+  }
 }
 
 // Bytes of the partials of `chunks` chunks (of all units together), each of a unit's query heads.
@@ -237,7 +250,7 @@ int dta_cache_read(const dta_cache_read_args* a, void* stream) {
 // device, and never less for more keys (a caller may size it for the capacity once).
 size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
   dta::CacheDecodeParams p;
-  if (decode_setup(a, &p, 1) != DTA_OK) return 0;
+  if (decode_setup(a, &p) != DTA_OK) return 0;
   const long long units = (long long)p.B * p.Hkv;
   return partial_bytes(a, units * dense_chunks_max(a->n_keys, units, a->cache.head_dim)) +
          partial_bytes(a, sparse_chunks_max(p.sink, p.window, units, a->cache.head_dim));
@@ -245,7 +258,7 @@ size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
 
 int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
   dta::CacheDecodeParams p;
-  int st = decode_setup(a, &p, 1);
+  int st = decode_setup(a, &p);
   if (st != DTA_OK) return st;
   if (!a->q || (!a->dense_out && !a->sparse_out)) return DTA_ERR_INVALID_ARG;
   if (!aligned(a->q, 16) || !aligned(a->dense_out, 16) || !aligned(a->sparse_out, 16)) return DTA_ERR_ALIGNMENT;
@@ -254,7 +267,7 @@ int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
   if (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)) return DTA_ERR_WORKSPACE;
   int sms = 0;
   if ((st = dta::check_device(&sms)) != DTA_OK) return st;
-  if ((st = decode_setup(a, &p, sms)) != DTA_OK) return st;  // chunking for this device
+  decode_plan(a, &p, sms);
   p.q = reinterpret_cast<const __nv_bfloat16*>(a->q);
   p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
   p.set[0].partials = reinterpret_cast<float*>(a->workspace);
