@@ -77,8 +77,8 @@ int sparse_chunk(long long sink, long long window, long long units, long long sl
     const long long steps = f * st, c = steps * kChunkStep, k = ceil_div(sink, c) + ceil_div(window, c);
     if (units * k > kSparseWaves * slots && steps != longest) continue;
     const long long sum = ceil_div(sink, kChunkStep) + ceil_div(window, kChunkStep) + k * kRampSteps;
-    const long long cost = (units * k <= slots ? 2 * (steps + kRampSteps) : 2 * units * sum / slots + steps + kRampSteps) +
-                           (k > 16 ? 4 : 0);
+    const long long own = steps + kRampSteps;  // (costs count half steps)
+    const long long cost = (units * k <= slots ? 2 * own : 2 * units * sum / slots + own) + (k > 16 ? 4 : 0);
     if (best_cost < 0 || cost < best_cost) {
       best = steps;
       best_cost = cost;
@@ -275,7 +275,8 @@ int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {
                                                  partial_bytes(a, (long long)p.B * p.Hkv * p.set[0].n_launched));
   p.out[0] = reinterpret_cast<__nv_bfloat16*>(a->dense_out);
   p.out[1] = reinterpret_cast<__nv_bfloat16*>(a->sparse_out);
-  const cudaError_t e = dta::launch_cache_decode(p, a->cache.head_dim, a->cache.format, reinterpret_cast<cudaStream_t>(stream));
+  const cudaError_t e = dta::launch_cache_decode(p, a->cache.head_dim, a->cache.format,
+                                                 reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? (int)DTA_OK : dta::fail_cuda(e);
 }
 

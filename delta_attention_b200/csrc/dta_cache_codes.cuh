@@ -19,7 +19,9 @@ namespace dta {
 
 // 2^(u - 127) for a scale byte; u = 0 (a block nothing was written to) is 2^-127.
 __device__ __forceinline__ float cache_scale(int u) {
-  return u == 0 ? __uint_as_float(0x00400000u) : u == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)u << 23);
+  return u == 0     ? __uint_as_float(0x00400000u)
+         : u == 255 ? __uint_as_float(0x7fc00000u)
+                    : __uint_as_float((uint32_t)u << 23);
 }
 // 2^(127 - u), the factor that a written value is multiplied by (1 <= u <= 253).
 __device__ __forceinline__ float cache_inv_scale(int u) { return __uint_as_float((uint32_t)(254 - u) << 23); }

@@ -13,7 +13,7 @@
 // by a power of two so that the largest element lies in [2^14, 2^15) (exact down to
 // 2^-29 of it); products and sums in fp32.  (The 8-bit mma.sync of this type converts
 // to fp16 itself: the kernel ran 25% more instructions with it.)  int8: codes as they
-// are, the query as a 16-bit integer, 32512 / max|q| times q (off by at most 2^-16 of
+// are, the query as a 16-bit integer, 32512 / max|q| times q (off by at most 1/65024 of
 // the largest element), in two 8-bit parts; products and sums in integers.  That costs no
 // conversion: 347 instructions for 16 keys, 364 to 398 with codes converted to fp16.
 //
@@ -34,19 +34,10 @@
 
 namespace dta {
 
-#ifndef DTA_CD_KEYS
-#define DTA_CD_KEYS 32
-#endif
-#ifndef DTA_CD_STAGES
-#define DTA_CD_STAGES 3
-#endif
-#ifndef DTA_CD_WARPS
-#define DTA_CD_WARPS 4
-#endif
-constexpr int CD_WARPS = DTA_CD_WARPS;
+constexpr int CD_WARPS = 4;
 constexpr int CD_THREADS = CD_WARPS * 32;
-constexpr int CD_KEYS = DTA_CD_KEYS;      // keys per step of a warp
-constexpr int CD_STAGES = DTA_CD_STAGES;  // steps in flight per warp
+constexpr int CD_KEYS = 32;   // keys per step of a warp
+constexpr int CD_STAGES = 3;  // steps in flight per warp
 static_assert(CD_WARPS * CD_KEYS == CACHE_STEP, "the host counts the same steps");
 constexpr float CD_SHIFT = 14.f;  // log2 of the factor that the fp16 weights carry
 
@@ -77,6 +68,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+
+// Live keys of sequence b.
 __device__ __forceinline__ int cd_live(const CacheDecodeParams& p, int b) {
   if (!p.n_keys_dev) return p.n_keys;
   return min(max(p.n_keys_dev[b * p.len_step], 0), p.n_keys);
@@ -184,10 +177,19 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
 // The grid's y covers the dense set's chunks and then the sparse set's, so a call
 // that wants both rows is one launch, whose short sparse chunks start last (and find
 // the sink and window in L2); its x the (batch, KV head) pairs.  CLU: the y extent is
-// one thread-block cluster per pair, and the
-// cluster merges its chunks' partials through distributed shared memory; else they
-// go to global memory and cache_merge_kernel merges them.  Both merge in one order,
-// so a sparse row is the same bit for bit whichever way it was launched.
+// one thread-block cluster per pair, and the cluster merges its chunks' partials through
+// distributed shared memory; else they go to global memory and cache_merge_kernel
+// merges them.  Both merge in one order, so a sparse row is the same bit for bit
+// whichever way it was launched.
+//
+// Why this shape.  At 8 bits a key costs half the memory time that it costs at 16, so
+// the instructions per key decide nearly as much as the memory does: 257 for 16 keys
+// (e4m3; 64 of them convert V and K), and the kernel without its copies takes 0.6 of
+// the time of one without its products.  Hence rings per warp (no barrier in the loop),
+// 32 keys a step, maxima that move by vote, and two CTAs of 4 warps per SM with 16 KB per
+// warp on the way; 12 warps with 8 KB each, 16-key steps, and K and V in rings of their own
+// were slower.  131072 keys, 8 KV heads x 4 queries, d 128, e4m3: 45.9 us with the merge,
+// 5.8 TB/s (the copies alone take 43.4); 4 x 65536: 82 us, 6.5 TB/s.
 template <int HD, int FMT, bool CLU>
 __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_constant__ CacheDecodeParams p) {
   constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16, NG = CD_KEYS / CACHE_GROUP;
@@ -206,8 +208,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
 
   if (!CLU && k0 >= k1) {  // no keys: an empty partial (its o is not read)
     if (threadIdx.x < G)
-      *reinterpret_cast<float4*>(S.partials + ((long long)(b * p.H + hk * G + threadIdx.x) * S.n_launched + chunk) * (4 + HD)) =
-          make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      *reinterpret_cast<float4*>(S.partials + ((long long)(b * p.H + hk * G + threadIdx.x) * S.n_launched + chunk) *
+                                                  (4 + HD)) = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     return;
   }
 
@@ -386,7 +388,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mma_f16(s[q], e4m3_half2((uint16_t)(w0[i] & 0xffffu)), e4m3_half2((uint16_t)(w1[i] & 0xffffu)),
-                    e4m3_half2((uint16_t)(w0[i] >> 16)), e4m3_half2((uint16_t)(w1[i] >> 16)), qb[c][i][0], qb[c][i][1]);
+                    e4m3_half2((uint16_t)(w0[i] >> 16)), e4m3_half2((uint16_t)(w1[i] >> 16)), qb[c][i][0],
+                    qb[c][i][1]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
@@ -456,7 +459,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       }
     }
     const float2 mu = make_float2(m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]);
-    const float2 ru = make_float2(r[0] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[0], r[1] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[1]);
+    const float2 ru = make_float2(r[0] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[0],
+                                  r[1] == -INFINITY ? CD_SHIFT : CD_SHIFT - r[1]);
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const float2 off = add2(make_float2(ve[q], ve[q]), ru);

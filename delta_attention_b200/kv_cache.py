@@ -64,6 +64,10 @@ class QuantizedKV:
         self.device = k.device
         self.index = k.device.index if k.device.type == "cuda" else None
         self.workspace_bytes = {}  # of cache_decode, by (heads, window, sink)
+        if self.index is not None:
+            from .ops import error_word
+
+            self.error_word = error_word(self.device)  # (here, not in a call that a graph may be capturing)
         # the C ABI's argument structs with this cache filled in; each call copies one
         self._write_args, self._read_args, self._decode_args = CacheWriteArgs(), CacheReadArgs(), CacheDecodeArgs()
         for a in (self._write_args, self._read_args, self._decode_args):

@@ -15,6 +15,7 @@ caller synchronises anyway) and raises ``DtaError(DTA_ERR_KERNEL_TIMEOUT)``.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -322,16 +323,12 @@ def _decode_workspace(nbytes: int, device) -> torch.Tensor:
     runs once per layer and token, so a fresh allocation per call would cost
     more host time than the kernel.  Calls on one stream are ordered, so they
     may share it.  (During CUDA graph capture a private buffer is used.)"""
-    return _stream_workspace(nbytes, _device_index(device), _stream())
-
-
-def _stream_workspace(nbytes: int, index: int, stream: int) -> torch.Tensor:
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return _workspace(nbytes, torch.device("cuda", index))
-    key = (index, stream)
+    if torch.cuda.is_current_stream_capturing():
+        return _workspace(nbytes, device)
+    key = (_device_index(device), _stream())
     ws = _decode_ws.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _workspace(nbytes, torch.device("cuda", index))
+        ws = _workspace(nbytes, device)
         _decode_ws[key] = ws
     return ws
 
@@ -462,6 +459,22 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_cache_ws = {}
+_cache_ws_lock = threading.Lock()
+
+
+def _cache_workspace(nbytes: int, index: int, stream: int) -> torch.Tensor:
+    """As :func:`_decode_workspace`.  The lock is held until the call's launches
+    are queued: two host threads on one stream would otherwise interleave the
+    launches of two calls that share the workspace."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return _workspace(nbytes, torch.device("cuda", index))
+    ws = _cache_ws.get((index, stream))
+    if ws is None or ws.numel() < nbytes:
+        ws = _cache_ws[(index, stream)] = _workspace(nbytes, torch.device("cuda", index))
+    return ws
+
+
 def _device_list(t: torch.Tensor, what: str, cache: QuantizedKV) -> int:
     if t.dtype != torch.int32 or t.device != cache.device or t.numel() not in (1, cache.batch) or \
             not t.is_contiguous():
@@ -523,8 +536,7 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, le
     k, a.k_new_stride_b, a.k_new_stride_h, a.k_new_stride_s = _in_place(k)
     v, a.v_new_stride_b, a.v_new_stride_h, a.v_new_stride_s = _in_place(v)
     a.k_new, a.v_new = k.data_ptr(), v.data_ptr()
-    word = _error_words.get(cache.index)
-    a.error_word = (error_word(cache.device) if word is None else word).data_ptr()
+    a.error_word = cache.error_word.data_ptr()
     _check_status(lib().dta_cache_write(ctypes.byref(a), _raw_stream(cache.index)), "dta_cache_write")
     if check:
         check_errors(cache.device)
@@ -618,9 +630,11 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     size = cache.workspace_bytes.get((H, a.window, a.sink))
     if size is None:
         size = cache.workspace_bytes[(H, a.window, a.sink)] = _cache_workspace_bytes(a, cache)
-    ws = _stream_workspace(size, cache.index, stream)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check_status(L.dta_cache_decode(ctypes.byref(a), stream), "dta_cache_decode")
+    with _cache_ws_lock:
+        ws = _cache_workspace(size, cache.index, stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        status = L.dta_cache_decode(ctypes.byref(a), stream)
+    _check_status(status, "dta_cache_decode")
     return dense, sparse
 
 

@@ -212,4 +212,5 @@ def test_oracle_appending_stays_within_one_rounding(fmt):
         assert torch.equal(once[normal], step[normal]) and (once - step).abs().max() <= 2.0 ** -9
     err = (orc.values(step[None], s2[None], 64)[0] - x.double()).abs()
     scale = 2.0 ** (int(s2[0]) - 127)
-    assert (err <= (scale if fmt == "int8" else torch.maximum(x.double().abs() * 2.0 ** -4, torch.tensor(scale * 2.0 ** -9)))).all()
+    most = scale if fmt == "int8" else torch.maximum(x.double().abs() * 2.0 ** -4, torch.tensor(scale * 2.0 ** -9))
+    assert (err <= most).all()

@@ -12,7 +12,7 @@ off_j = scaling * (c |q| . |k_j| + e max|q| sum|k_j|):
   sum w off |v| + (sum w off) W   the scores, off by off_j, move a weight and the sum of the weights
                          relatively by as much.  c = (d + 6) 2^-23: sums over d terms in fp32 (d steps,
                          and 6 more for the products with the scales and log2 e).  e: the query's own
-                         rounding, 2^-29 for e4m3 (fp16, scaled) and 2^-16 for int8 (16 bits)
+                         rounding, 2^-29 for e4m3 (fp16, scaled) and 1/65024 for int8 (half a step of 1/32512)
   2^-13 W                sums of weights and products in fp32 (at most 2^9 steps of 2^-23 each in a warp's
                          share, and the merges), exp2's 2^-22, the maxima's shifts
 """
@@ -155,7 +155,8 @@ def test_write_special_values(fmt):
     d, block = 64, 16
     q = orc.QMAX[fmt]
     rows = torch.zeros(12 * block, d)
-    for i, x in enumerate((0.0, q, math.nextafter(q, 1e9), q * 2.0 ** -120, 1e-44, 3.3895e38, 3.4028e38, 1.0, 2.0 ** -126)):
+    for i, x in enumerate((0.0, q, math.nextafter(q, 1e9), q * 2.0 ** -120, 1e-44, 3.3895e38, 3.4028e38, 1.0,
+                           2.0 ** -126)):
         rows[i * block, 3] = torch.tensor(x, dtype=torch.float64).float()
         rows[i * block + 5, 7] = -rows[i * block, 3] * 0.37
     rows[9 * block + 2] = torch.linspace(-q, q, d)
@@ -229,7 +230,8 @@ def _check_rows(got, q, cache, n, window, sink, sparse, what, scaling=None):
     kv = [orc.values(c, s, cache.block) for c, s in _state(cache)]
     for i in range(cache.batch):
         out, spread, slack = orc.attend(q[i, :, 0].float().cpu(), kv[0][i], kv[1][i], n[i], scaling, window, sink,
-                                        sparse, (d + 6) * 2.0 ** -23, 2.0 ** (-16 if cache.format == "int8" else -29))
+                                        sparse, (d + 6) * 2.0 ** -23,
+                                        1 / 65024 if cache.format == "int8" else 2.0 ** -29)
         vmax = kv[1][i, :, :n[i]].abs().amax().item() if n[i] else 0.0
         tol = 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2.0 ** -13) * spread + n[i] * 2.0 ** -38 * vmax + slack
         err = (got[i, 0].float().cpu().double() - out).abs()
@@ -446,6 +448,79 @@ def test_calls_on_two_streams():
     for i in range(2):
         for x in got[i]:
             assert torch.equal(x[0], want[i][0]) and torch.equal(x[1], want[i][1])
+
+
+def test_calls_of_two_threads_on_one_stream():
+    """Two host threads that decode on the same stream: each call's launches
+    stay together, so the shared workspace holds one call's partials at a time."""
+    import threading
+    ops = _ops()
+    cache = _filled(1, 8, 20000, 64, "e4m3", 64, [20000], seed=16)  # (long enough for a merge launch)
+    qs = [_rows(1, 16, 1, 64, torch.bfloat16, i).cuda() for i in range(2)]
+    want = [ops.cache_decode(q, cache, window=500, sink=64) for q in qs]
+    got, stream = [[], []], torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got[i].append(ops.cache_decode(qs[i], cache, window=500, sink=64))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 50
+        for x in got[i]:
+            assert torch.equal(x[0], want[i][0]) and torch.equal(x[1], want[i][1])
+
+
+def test_no_keys_at_all():
+    """A host count of zero, and reads and writes of nothing."""
+    ops = _ops()
+    cache = _cache(2, 2, 100, 64, "e4m3", 16, seed=1)
+    before = _raw(cache)
+    dense, sparse = ops.cache_decode(_rows(2, 4, 1, 64, torch.bfloat16, 1).cuda(), cache, window=10, sink=2, n_keys=0)
+    assert not dense.any() and not sparse.any()
+    empty = torch.empty(2, 2, 0, 64, dtype=torch.bfloat16, device="cuda")
+    ops.cache_write(cache, empty, empty, pos=100, check=True)
+    k, v = ops.cache_read(cache, n_keys=0, start=100)
+    assert tuple(k.shape) == tuple(v.shape) == (2, 2, 0, 64)
+    assert all(torch.equal(x, y) for x, y in zip(before, _raw(cache)))
+
+
+def test_ops_refuse_mismatched_tensors():
+    """Refused before any launch: the cache and the outputs are not touched."""
+    ops = _ops()
+    cache = _cache(2, 2, 100, 64, "int8", 16, seed=1)
+    x = _rows(2, 2, 3, 64, torch.bfloat16, 1).cuda()
+    q = _rows(2, 4, 1, 64, torch.bfloat16, 1).cuda()
+    n = torch.tensor([3, 3], dtype=torch.int32).cuda()
+    for call in (lambda: ops.cache_write(cache, x[:1], x[:1], pos=0),
+                 lambda: ops.cache_write(cache, x, x[:, :, :2], pos=0),
+                 lambda: ops.cache_write(cache, x, x.half(), pos=0),
+                 lambda: ops.cache_write(cache, x.int(), x.int(), pos=0),
+                 lambda: ops.cache_write(cache, x, x, pos=98), lambda: ops.cache_write(cache, x, x, pos=-1),
+                 lambda: ops.cache_write(cache, x.cpu(), x.cpu(), pos=0),
+                 lambda: ops.cache_write(cache, x, x, pos=n.long()), lambda: ops.cache_write(cache, x, x, pos=n.cpu()),
+                 lambda: ops.cache_write(cache, x, x, pos=0, lengths=n.repeat(2)),
+                 lambda: ops.cache_read(cache, n_keys=101), lambda: ops.cache_read(cache, start=-1),
+                 lambda: ops.cache_read(cache, dtype=torch.float64), lambda: ops.cache_read(cache, out=(x, x)),
+                 lambda: ops.cache_decode(q[:1], cache, window=1, sink=1),
+                 lambda: ops.cache_decode(q.expand(2, 4, 2, 64), cache, window=1, sink=1),
+                 lambda: ops.cache_decode(q.cpu(), cache, window=1, sink=1),
+                 lambda: ops.cache_decode(q, cache, window=1, sink=1, n_keys=101),
+                 lambda: ops.cache_decode(q, cache, window=1, sink=1, n_keys_dev=n.float()),
+                 lambda: ops.cache_decode(q, cache, window=1, sink=1, want_dense=False, want_sparse=False)):
+        with pytest.raises(ValueError):
+            call()
+    from delta_attention_b200._lib import DtaError
+    for heads in (3, 18):  # not a multiple of the KV heads; more than 8 to one
+        with pytest.raises(DtaError, match="SHAPE"):
+            ops.cache_decode(_rows(2, heads, 1, 64, torch.bfloat16, 1).cuda(), cache, window=1, sink=1)
 
 
 def test_write_read_attend_together():
