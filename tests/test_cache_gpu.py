@@ -267,7 +267,8 @@ def test_decode(fmt, b, H, Hkv, d, block, cap, n, window, sink):
     alone, none = ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_sparse=False)
     assert none is None
     _check_rows(alone, q, cache, n, window, sink, False, "dense alone")
-    assert torch.equal(ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_dense=False)[1], sparse)
+    alone = ops.cache_decode(q, cache, window=window, sink=sink, n_keys_dev=live, want_dense=False)
+    assert alone[0] is None and torch.equal(alone[1], sparse)
     if len(set(n)) == 1:  # a host count
         dense, sparse = ops.cache_decode(q, cache, window=window, sink=sink, n_keys=n[0])
         _check_rows(dense, q, cache, n, window, sink, False, "dense, host count")
@@ -428,6 +429,42 @@ def test_step_captured_and_replayed():
         want = ops.cache_decode(qs[i], caches[0], window=40, sink=4, n_keys_dev=n)
         assert torch.equal(outs[i % 2][0], want[0]) and torch.equal(outs[i % 2][1], want[1]), i
     ops.check_errors()
+
+
+def test_first_calls_within_a_capture():
+    """A process whose first calls of these kernels are captured (no eager run
+    before): the replays do what the eager calls then do."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from delta_attention_b200 import ops
+from delta_attention_b200.kv_cache import QuantizedKV
+caches = [QuantizedKV.allocate(1, 2, n, 64, format=f, block=16) for n, f in ((6000, 'e4m3'), (300, 'int8'))]
+g = torch.Generator(device='cuda').manual_seed(0)
+k, v = (torch.randn(1, 2, 300, 64, generator=g, device='cuda') for _ in range(2))
+q = torch.randn(1, 8, 1, 64, generator=g, device='cuda').bfloat16()
+live = torch.tensor([300], dtype=torch.int32, device='cuda')
+def step():
+    out = []
+    for c in caches:
+        ops.cache_write(c, k, v, pos=0)
+        out += ops.cache_decode(q, c, window=100, sink=9, n_keys_dev=live)
+        out += ops.cache_read(c, n_keys=300)
+    return out
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in got]
+for x, y in zip(got, step()):
+    assert x.abs().sum() > 0 and torch.equal(x, y)
+ops.check_errors()
+print('same')
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
 
 
 def test_calls_on_two_streams():
