@@ -48,7 +48,8 @@ struct CacheReadParams {
 constexpr int CACHE_GROUP = 16;
 
 // Keys in one step of a CTA of the decode kernel, and what its start and end cost, in steps.
-constexpr int CACHE_STEP = 128, CACHE_RAMP_STEPS = 3;
+constexpr int cache_step(int head_dim) { return head_dim == 128 ? 128 : 256; }
+constexpr int CACHE_RAMP_STEPS = 3;
 
 struct CacheDecodeSet {
   int chunk;               // keys per chunk, a multiple of CACHE_GROUP

@@ -52,12 +52,11 @@ int check_list(const int32_t* list, int n, int batch, int* step) {
 
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-constexpr int kChunkStep = dta::CACHE_STEP;  // one step of a CTA's warps
 constexpr int kRampSteps = dta::CACHE_RAMP_STEPS;
 constexpr int kMaxSms = 160;  // SMs that are counted at most (a B200 has 148)
 
 // CTAs of the partial kernel that are resident on an SM (shared memory bounds them).
-int resident_ctas(int head_dim) { return head_dim == 128 ? 2 : 4; }
+constexpr int kResidentCtas = 2;
 
 // Chunk of the sparse set, by the estimated time of its CTAs in steps: one that all are
 // resident with costs its own steps and kRampSteps; more of them the sum of their
@@ -69,14 +68,14 @@ constexpr int kSparseSteps[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
 constexpr int kSparseWaves = 4;  // chunks that would take more waves are not tried
 constexpr long long kSparseKeys = 1 << 23;  // windows beyond this take longer chunks (a launch has 65535 at most)
 
-int sparse_chunk(long long sink, long long window, long long units, long long slots) {
+int sparse_chunk(long long sink, long long window, long long units, long long slots, int step) {
   const long long f = sink + window > kSparseKeys ? ceil_div(sink + window, kSparseKeys) : 1;
   const long long longest = f * kSparseSteps[sizeof(kSparseSteps) / sizeof(int) - 1];
   long long best = longest, best_cost = -1;
   for (int st : kSparseSteps) {
-    const long long steps = f * st, c = steps * kChunkStep, k = ceil_div(sink, c) + ceil_div(window, c);
+    const long long steps = f * st, c = steps * step, k = ceil_div(sink, c) + ceil_div(window, c);
     if (units * k > kSparseWaves * slots && steps != longest) continue;
-    const long long sum = ceil_div(sink, kChunkStep) + ceil_div(window, kChunkStep) + k * kRampSteps;
+    const long long sum = ceil_div(sink, step) + ceil_div(window, step) + k * kRampSteps;
     const long long own = steps + kRampSteps;  // (costs count half steps)
     const long long cost = (units * k <= slots ? 2 * own : 2 * units * sum / slots + own) + (k > 16 ? 4 : 0);
     if (best_cost < 0 || cost < best_cost) {
@@ -84,12 +83,12 @@ int sparse_chunk(long long sink, long long window, long long units, long long sl
       best_cost = cost;
     }
   }
-  return (int)best * kChunkStep;
+  return (int)best * step;
 }
 // At most this many sparse chunks of all units, on any device and for any smaller sink and window.
-long long sparse_chunks_max(long long sink, long long window, long long units, int head_dim) {
-  const long long few = (long long)kSparseWaves * kMaxSms * resident_ctas(head_dim);
-  const long long chunks = ceil_div(sink + window, 32 * kChunkStep), most = kSparseKeys / (32 * kChunkStep);
+long long sparse_chunks_max(long long sink, long long window, long long units) {
+  const long long few = (long long)kSparseWaves * kMaxSms * kResidentCtas;
+  const long long chunks = ceil_div(sink + window, 32 * 128), most = kSparseKeys / (32 * 128);
   const long long many = units * ((chunks < most ? chunks : most) + 2);
   return few > many ? few : many;
 }
@@ -111,8 +110,8 @@ long long sparse_chunks_max(long long sink, long long window, long long units, i
 constexpr int kWaves = 4;
 
 int dense_chunk(long long n, long long units, long long sparse_ctas, long long sparse_steps, bool ragged,
-                long long slots) {
-  if (n <= kChunkStep) return kChunkStep;
+                long long slots, int step) {
+  if (n <= step) return step;
   if (sparse_ctas == 0 && slots > 1) slots = slots * 7 / 8;
   const long long sparse_cost = sparse_steps + kRampSteps;
   long long best = 0, best_cost = 0;
@@ -120,14 +119,14 @@ int dense_chunk(long long n, long long units, long long sparse_ctas, long long s
     if (sparse_ctas == 0 && i % 3 != 0) continue;
     const long long room = i % 3 * (sparse_ctas < slots / 2 ? sparse_ctas : slots / 2) / 2;
     const long long places = (i / 3 + 1) * slots - room, k = places / units > 0 ? places / units : 1;
-    const long long steps = ceil_div(n, k * kChunkStep), cost = steps + kRampSteps;
-    const long long ctas = ceil_div(ceil_div(n, steps * kChunkStep) * units, ragged ? 2 : 1);
+    const long long steps = ceil_div(n, k * step), cost = steps + kRampSteps;
+    const long long ctas = ceil_div(ceil_div(n, steps * step) * units, ragged ? 2 : 1);
     const long long waves = ceil_div(ctas, slots);
     const long long beside = (waves * slots - ctas) * (cost / sparse_cost);
     const long long after = sparse_ctas > beside ? ceil_div(sparse_ctas - beside, slots) * sparse_cost : 0;
     const long long total = waves * cost + after;
     if (best == 0 || total < best_cost) {
-      best = steps * kChunkStep;
+      best = steps * step;
       best_cost = total;
     }
   }
@@ -135,8 +134,8 @@ int dense_chunk(long long n, long long units, long long sparse_ctas, long long s
 }
 
 // At most this many dense chunks per unit, on any device.
-long long dense_chunks_max(long long n, long long units, int head_dim) {
-  const long long k = (long long)kWaves * kMaxSms * resident_ctas(head_dim) / units, shortest = ceil_div(n, kChunkStep);
+long long dense_chunks_max(long long n, long long units, int step) {
+  const long long k = (long long)kWaves * kMaxSms * kResidentCtas / units, shortest = ceil_div(n, step);
   return k < 1 ? 1 : k < shortest ? k : shortest;
 }
 
@@ -164,18 +163,19 @@ int decode_setup(const dta_cache_decode_args* a, dta::CacheDecodeParams* p) {
 // The chunks of the sets that are wanted, for a device of `sms` SMs.
 void decode_plan(const dta_cache_decode_args* a, dta::CacheDecodeParams* p, int sms) {
   const long long units = (long long)p->B * p->Hkv, n = p->n_keys;
-  const long long slots = (sms < kMaxSms ? sms : kMaxSms) * resident_ctas(a->cache.head_dim);
+  const long long slots = (sms < kMaxSms ? sms : kMaxSms) * kResidentCtas;
+  const int step = dta::cache_step(a->cache.head_dim);
   const bool ragged = p->n_keys_dev && p->len_step;
   p->clusters = !(ragged && a->dense_out);  // an empty chunk would hold its place until its cluster is done
   if (a->sparse_out) {
-    const int c = sparse_chunk(p->sink, p->window, units, slots);
+    const int c = sparse_chunk(p->sink, p->window, units, slots, step);
     p->set[1].chunk = c;
     p->set[1].n_sink_chunks = (int)ceil_div(p->sink, c);
     p->set[1].n_launched = p->set[1].n_sink_chunks + (int)ceil_div(p->window, c);
     if (p->set[1].n_launched < 1) p->set[1].n_launched = 1;  // no keys: one empty partial
   }
   if (a->dense_out) {
-    const int c = dense_chunk(n, units, units * p->set[1].n_launched, p->set[1].chunk / kChunkStep, ragged, slots);
+    const int c = dense_chunk(n, units, units * p->set[1].n_launched, p->set[1].chunk / step, ragged, slots, step);
     p->set[0].chunk = c;
     p->set[0].n_launched = n > 0 ? (int)ceil_div(n, c) : 1;
   }
@@ -252,8 +252,8 @@ size_t dta_cache_decode_workspace_size(const dta_cache_decode_args* a) {
   dta::CacheDecodeParams p;
   if (decode_setup(a, &p) != DTA_OK) return 0;
   const long long units = (long long)p.B * p.Hkv;
-  return partial_bytes(a, units * dense_chunks_max(a->n_keys, units, a->cache.head_dim)) +
-         partial_bytes(a, sparse_chunks_max(p.sink, p.window, units, a->cache.head_dim));
+  return partial_bytes(a, units * dense_chunks_max(a->n_keys, units, dta::cache_step(a->cache.head_dim))) +
+         partial_bytes(a, sparse_chunks_max(p.sink, p.window, units));
 }
 
 int dta_cache_decode(const dta_cache_decode_args* a, void* stream) {

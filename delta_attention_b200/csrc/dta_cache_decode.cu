@@ -36,9 +36,9 @@ namespace dta {
 
 constexpr int CD_WARPS = 4;
 constexpr int CD_THREADS = CD_WARPS * 32;
-constexpr int CD_KEYS = 32;   // keys per step of a warp
+template <int HD>
+constexpr int CD_KEYS = cache_step(HD) / CD_WARPS;  // keys per step of a warp: 4 KB of K and of V
 constexpr int CD_STAGES = 3;  // steps in flight per warp
-static_assert(CD_WARPS * CD_KEYS == CACHE_STEP, "the host counts the same steps");
 constexpr float CD_SHIFT = 14.f;  // log2 of the factor that the fp16 weights carry
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -152,7 +152,7 @@ __device__ __forceinline__ int cd_swizzle(int row, int piece) {
 }
 template <int HD>
 __host__ __device__ constexpr int cd_smem() {
-  return CD_WARPS * CD_STAGES * 2 * CD_KEYS * HD;
+  return CD_WARPS * CD_STAGES * 2 * CD_KEYS<HD> * HD;
 }
 __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&w)[4]) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
@@ -192,7 +192,8 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
 // 5.8 TB/s (the copies alone take 43.4); 4 x 65536: 82 us, 6.5 TB/s.
 template <int HD, int FMT, bool CLU>
 __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_constant__ CacheDecodeParams p) {
-  constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16, NG = CD_KEYS / CACHE_GROUP;
+  constexpr int KEYS = CD_KEYS<HD>, NG = KEYS / CACHE_GROUP;
+  constexpr int KP = HD / 64, VW = HD / 32, NJ = HD / 16;
   extern __shared__ __align__(128) uint8_t cd_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -221,11 +222,11 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
 
   // ---- copies: lane -> piece lane % PC of rows lane / PC, + 32 / PC, ... ----
   constexpr int PC = HD / 16, RL = 32 / PC;  // pieces per row, rows per pass
-  constexpr int STAGE = 2 * CD_KEYS * HD;
+  constexpr int STAGE = 2 * KEYS * HD;
   const uint32_t ring = smem_u32(cd_ring) + warp * CD_STAGES * STAGE;
   const int cr = lane / PC, cp = lane % PC;
-  const int a0 = (k0 & ~(CACHE_GROUP - 1)) + warp * CD_KEYS;
-  constexpr int STRIDE = CD_WARPS * CD_KEYS;
+  const int a0 = (k0 & ~(CACHE_GROUP - 1)) + warp * KEYS;
+  constexpr int STRIDE = CD_WARPS * KEYS;
   const int steps = k1 > a0 ? (k1 - a0 + STRIDE - 1) / STRIDE : 0;
   // shared-memory offsets of this lane's pieces of its first and second row (the
   // permutation repeats after two passes)
@@ -237,31 +238,31 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     const uint32_t dst = ring + slot * STAGE;
     const uint8_t* ksrc = kc + (long long)(base + cr) * kss + cp * 16;
     const uint8_t* vsrc = vc + (long long)(base + cr) * vss + cp * 16;
-    if (base >= k0 && base + CD_KEYS <= k1) {
+    if (base >= k0 && base + KEYS <= k1) {
       if (packed) {  // rows follow one another: every offset is a constant
 #pragma unroll
-        for (int i = 0; i < CD_KEYS / RL; ++i)
+        for (int i = 0; i < KEYS / RL; ++i)
           cp_async_16(dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD, ksrc + i * RL * HD, 16u);
 #pragma unroll
-        for (int i = 0; i < CD_KEYS / RL; ++i)
-          cp_async_16(dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD + CD_KEYS * HD, vsrc + i * RL * HD, 16u);
+        for (int i = 0; i < KEYS / RL; ++i)
+          cp_async_16(dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD + KEYS * HD, vsrc + i * RL * HD, 16u);
       } else {
 #pragma unroll
-        for (int i = 0; i < CD_KEYS / RL; ++i) {
+        for (int i = 0; i < KEYS / RL; ++i) {
           const uint32_t off = dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD;
           cp_async_16(off, ksrc + i * RL * kss, 16u);
-          cp_async_16(off + CD_KEYS * HD, vsrc + i * RL * vss, 16u);
+          cp_async_16(off + KEYS * HD, vsrc + i * RL * vss, 16u);
         }
       }
     } else {
       // rows outside the chunk are filled with zeros (a masked value must not be NaN: 0 * NaN)
 #pragma unroll
-      for (int i = 0; i < CD_KEYS / RL; ++i) {
+      for (int i = 0; i < KEYS / RL; ++i) {
         const int key = base + cr + i * RL;
         const bool ok = key >= k0 && key < k1;
         const uint32_t off = dst + (i & 1 ? c1 : c0) + (i >> 1) * 2 * RL * HD;
         cp_async_16(off, ok ? ksrc + i * RL * kss : kc + (long long)k0 * kss, ok ? 16u : 0u);
-        cp_async_16(off + CD_KEYS * HD, ok ? vsrc + i * RL * vss : vc + (long long)k0 * vss, ok ? 16u : 0u);
+        cp_async_16(off + KEYS * HD, ok ? vsrc + i * RL * vss : vc + (long long)k0 * vss, ok ? 16u : 0u);
       }
     }
   };
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
   for (int c = 0; c < KP; ++c) ka[c] = g * HD + (cd_swizzle<HD>(g, KP * t + c) << 4);
 #pragma unroll
   for (int e = 0; e < 2; ++e)
-    va[e] = CD_KEYS * HD + (2 * t + e) * HD + (cd_swizzle<HD>(2 * t + e, HD == 128 ? g : g >> 1) << 4) +
+    va[e] = KEYS * HD + (2 * t + e) * HD + (cd_swizzle<HD>(2 * t + e, HD == 128 ? g : g >> 1) << 4) +
             (HD == 128 ? 0 : 8 * (g & 1));
 
   int slot = 0;
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       s[q][2] = y.x;
       s[q][3] = y.y;
     }
-    if (base < k0 || base + CD_KEYS > k1) {
+    if (base < k0 || base + KEYS > k1) {
 #pragma unroll
       for (int q = 0; q < NG; ++q)
 #pragma unroll
