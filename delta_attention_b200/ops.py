@@ -463,15 +463,17 @@ _cache_ws = {}
 _cache_ws_lock = threading.Lock()
 
 
-def _cache_workspace(nbytes: int, index: int, stream: int) -> torch.Tensor:
-    """As :func:`_decode_workspace`.  The lock is held until the call's launches
-    are queued: two host threads on one stream would otherwise interleave the
-    launches of two calls that share the workspace."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return _workspace(nbytes, torch.device("cuda", index))
-    ws = _cache_ws.get((index, stream))
-    if ws is None or ws.numel() < nbytes:
-        ws = _cache_ws[(index, stream)] = _workspace(nbytes, torch.device("cuda", index))
+def _cache_workspace(nbytes: int, index: int, stream: int):
+    """(tensor, address, bytes), kept as :func:`_decode_workspace` keeps one.  The
+    lock is held until the call's launches are queued: two host threads on one
+    stream would otherwise interleave the launches of two calls that share it."""
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
+    ws = None if capturing else _cache_ws.get((index, stream))
+    if ws is None or ws[2] < nbytes:
+        t = _workspace(nbytes, torch.device("cuda", index))
+        ws = (t, t.data_ptr(), t.numel())
+        if not capturing:
+            _cache_ws[(index, stream)] = ws
     return ws
 
 
@@ -511,15 +513,16 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, le
     ``check=True`` does that right after the launch)."""
     if not _is_current(cache):
         return _on_cache_device(cache_write, cache, cache, k, v, pos=pos, lengths=lengths, check=check)
-    if k.shape != v.shape or k.dim() != 4 or (k.shape[0], k.shape[1], k.shape[3]) != (
-            cache.batch, cache.n_kv_heads, cache.head_dim):
+    shape = k.shape
+    if v.shape != shape or len(shape) != 4 or shape[0] != cache.batch or shape[1] != cache.n_kv_heads or \
+            shape[3] != cache.head_dim:
         raise ValueError(f"k and v must be [{cache.batch}, {cache.n_kv_heads}, s, {cache.head_dim}], got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype not in _CACHE_TYPES or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be bf16, fp16 or fp32, got {k.dtype} and {v.dtype}")
     if k.device != cache.device or v.device != cache.device:
         raise ValueError(f"k and v must be on the cache's device {cache.device}")
-    s = k.shape[2]
+    s = shape[2]
     if s == 0:
         return
     a = CacheWriteArgs.from_buffer_copy(cache._write_args)
@@ -559,11 +562,11 @@ def cache_read(cache: QuantizedKV, *, n_keys: Optional[int] = None, start: int =
         raise ValueError(f"positions [{start}, {start + n}) are outside the cache of {cache.capacity}")
     if dtype not in _CACHE_TYPES:
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    shape = (cache.batch, cache.n_kv_heads, n, cache.head_dim)
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=cache.device),
-               torch.empty(shape, dtype=dtype, device=cache.device))
+        k = cache.k.new_empty(cache.batch, cache.n_kv_heads, n, cache.head_dim, dtype=dtype)
+        out = (k, torch.empty_like(k))
     else:
+        shape = (cache.batch, cache.n_kv_heads, n, cache.head_dim)
         for t in out:
             if tuple(t.shape) != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous():
                 raise ValueError(f"out must be two contiguous {shape} {dtype} tensors on {cache.device}")
@@ -619,10 +622,10 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     a.scaling = d ** -0.5 if scaling is None else float(scaling)
     dense = sparse = None
     if want_dense:
-        dense = q.new_empty((b, 1, H, d))
+        dense = q.new_empty(b, 1, H, d)
         a.dense_out = dense.data_ptr()
     if want_sparse:
-        sparse = q.new_empty((b, 1, H, d))
+        sparse = q.new_empty(b, 1, H, d)
         a.sparse_out = sparse.data_ptr()
     if n_keys_dev is not None:
         a.n_keys_dev, a.n_lengths = _device_list(n_keys_dev, "n_keys_dev", cache), n_keys_dev.numel()
@@ -631,8 +634,7 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     if size is None:
         size = cache.workspace_bytes[(H, a.window, a.sink)] = _cache_workspace_bytes(a, cache)
     with _cache_ws_lock:
-        ws = _cache_workspace(size, cache.index, stream)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        ws, a.workspace, a.workspace_bytes = _cache_workspace(size, cache.index, stream)
         status = L.dta_cache_decode(ctypes.byref(a), stream)
     _check_status(status, "dta_cache_decode")
     return dense, sparse
