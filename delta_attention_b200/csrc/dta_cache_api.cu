@@ -96,17 +96,17 @@ long long sparse_chunks_max(long long sink, long long window, long long units) {
 // Chunk of the dense set: the one with the least estimated time, in steps of a CTA.
 // 7/8 of the resident CTAs are used (the sparse ones take the rest where they are
 // wanted): the memory is saturated by them, and SMs that have one CTA instead of two
-// even out at the end (131072 keys, 8 KV heads: 47.1 us
-// with 256 CTAs, 48.6 with 296, 55 with 168; 4 x 65536: 82.1 with 256, 88.8 with 288,
-// 92 with 192).  With that many `slots`, w waves of them take k = w slots / units chunks
-// of each unit (a (batch, KV head)); a CTA costs its chunk's steps plus kRampSteps
-// for its start and end (a step takes 1.5 us while the memory is saturated).  The
-// sparse set's CTAs, if they are wanted too, come last: into the places that the
-// dense ones leave, else after them, so fewer chunks that leave them room are tried as
-// well.  Where sequences have lengths of their own, about half of the chunks are taken
-// to be empty.  (16 sequences of 8191 down to 0 keys, 8 KV heads: 29.6 us with 2048-key
-// chunks, 32.6 with 1024, 38.3 with 4096.  32761 keys, 8 KV heads of 8 queries, both
-// rows: 21.5 us with 1152, which leaves the sparse chunks room, 25.1 with 896.)
+// even out at the end (131072 keys, 8 KV heads: 47.1 us with 256 CTAs, 48.6 with 296, 55
+// with 168; 4 x 65536: 82.1 with 256, 88.8 with 288, 92 with 192).  With that many
+// `slots`, w waves of them take k = w slots / units chunks of each unit (a (batch, KV
+// head)); a CTA costs its chunk's steps plus kRampSteps for its start and end (a step
+// takes 1.5 us while the memory is saturated).  The sparse set's CTAs, if they are wanted
+// too, come last: into the places that the dense ones leave, else after them, so fewer
+// chunks that leave them room are tried as well.  Where sequences have lengths of their
+// own, about half of the chunks are taken to be empty.  (16 sequences of 8191 down to 0
+// keys, 8 KV heads: 29.6 us with 2048-key chunks, 32.6 with 1024, 38.3 with 4096.  32761
+// keys, 8 KV heads of 8 queries, both rows: 21.5 us with 1152, which leaves the sparse
+// chunks room, 25.1 with 896.)
 constexpr int kWaves = 4;
 
 int dense_chunk(long long n, long long units, long long sparse_ctas, long long sparse_steps, bool ragged,

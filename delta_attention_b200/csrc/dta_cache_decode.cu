@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       f = __uint_as_float((uint32_t)(127 + up) << 23);
       my_scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
     } else {
-      const float most = fmaxf(__uint_as_float(top), 0x1p-100f);  // (a head that is all smaller counts as zeros)
+      const float most = fmaxf(__uint_as_float(top), 0x1p-112f);  // (smaller heads would overflow f, and count as zeros)
       f = 32512.f / most;
       my_scale = p.scale_log2 * (most / 32512.f);
     }

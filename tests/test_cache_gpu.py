@@ -487,6 +487,36 @@ def test_calls_on_two_streams():
             assert torch.equal(x[0], want[i][0]) and torch.equal(x[1], want[i][1])
 
 
+def test_calls_from_another_current_device(monkeypatch):
+    """Where the cache's device is not the current one, an op runs again with it
+    current (here the check is made to say so once)."""
+    ops = _ops()
+    cache = _filled(1, 2, 100, 64, "e4m3", 64, [100], seed=12)
+    q = _rows(1, 4, 1, 64, torch.bfloat16, 4).cuda()
+    x = _rows(1, 2, 3, 64, torch.bfloat16, 4).cuda()
+    entered = []
+
+    def once(answers):
+        left = list(answers)
+        monkeypatch.setattr(ops, "_is_current", lambda c: left.pop(0))
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    want = ops.cache_decode(q, cache, window=10, sink=1)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    once([False, True])
+    got = ops.cache_decode(q, cache, window=10, sink=1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    once([False, True])
+    ops.cache_write(cache, x, x, pos=97)
+    once([False, True])
+    k, _ = ops.cache_read(cache, n_keys=3, start=97, dtype=torch.float32)
+    assert k.abs().sum() > 0 and entered == [0, 0, 0]
+
+
 def test_calls_of_two_threads_on_one_stream():
     """Two host threads that decode on the same stream: each call's launches
     stay together, so the shared workspace holds one call's partials at a time."""
