@@ -135,7 +135,8 @@ int dense_chunk(long long n, long long units, long long sparse_ctas, long long s
 
 // At most this many dense chunks per unit, on any device.
 long long dense_chunks_max(long long n, long long units, int step) {
-  const long long k = (long long)kWaves * kMaxSms * kResidentCtas / units, shortest = ceil_div(n, step);
+  const long long k = (long long)kWaves * kMaxSms * kResidentCtas / units;
+  const long long shortest = n > 0 ? ceil_div(n, step) : 1;  // (without keys: one empty chunk)
   return k < 1 ? 1 : k < shortest ? k : shortest;
 }
 

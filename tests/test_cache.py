@@ -174,6 +174,18 @@ def test_decode_workspace_size():
     assert L.dta_cache_decode_workspace_size(ctypes.byref(a)) == 0
 
 
+@pytest.mark.parametrize("batch,heads,d", [(1, 8, 128), (641, 1, 64), (643, 5, 128), (1283, 3, 64), (2001, 1, 128)])
+def test_decode_workspace_holds_empty_partials(batch, heads, d):
+    """Without keys each set still writes one partial per query head: 4 + d
+    words, the second set's behind the first's, rounded up to 256 bytes."""
+    L = _lib.lib()
+    a = _args(_lib.CacheDecodeArgs)
+    a.cache.batch, a.cache.n_kv_heads, a.cache.head_dim = batch, 1, d
+    a.n_heads, a.n_keys, a.window, a.sink = heads, 0, 0, 0
+    one = batch * heads * (4 + d) * 4
+    assert L.dta_cache_decode_workspace_size(ctypes.byref(a)) >= -(-one // 256) * 256 + one
+
+
 # ---- the oracle itself ------------------------------------------------------------------------------
 
 def test_oracle_rounding_is_torchs():
