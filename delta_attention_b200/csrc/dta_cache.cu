@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
   const int tg = threadIdx.x & (group - 1);
   const int per_cta = blockDim.x >> log_group;
   const int blk0 = (first >> p.log_block) + slab * per_cta;
-  if (len == 0 || (blk0 << p.log_block) >= end) return;  // (the whole CTA)
+  // the whole CTA is past the end (compared in blocks: their positions may pass 2^31)
+  if (len == 0 || blk0 > (end - 1) >> p.log_block) return;
   const int blk = blk0 + (threadIdx.x >> log_group);
   const int lo = blk << p.log_block;
   const int T = 1 << p.log_block, dr = group / RC;  // rows of a block, rows between a thread's pieces
