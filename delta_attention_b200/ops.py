@@ -615,10 +615,14 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
     n = cache.capacity if n_keys is None else int(n_keys)
     if not 0 <= n <= cache.capacity:
         raise ValueError(f"n_keys {n} is outside the cache of {cache.capacity}")
+    window, sink = int(window), int(sink)
+    if window < 0 or sink < 0:
+        raise ValueError(f"window {window} and sink {sink} must not be negative")
     a = CacheDecodeArgs.from_buffer_copy(cache._decode_args)
     q, a.q_stride_b, a.q_stride_h, _ = _in_place(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16))
     a.q = q.data_ptr()
-    a.n_heads, a.n_keys, a.window, a.sink = H, n, int(window), int(sink)
+    # (more than the cache holds means all of it; the struct's fields have 32 bits)
+    a.n_heads, a.n_keys, a.window, a.sink = H, n, min(window, cache.capacity), min(sink, cache.capacity)
     a.scaling = d ** -0.5 if scaling is None else float(scaling)
     dense = sparse = None
     if want_dense:

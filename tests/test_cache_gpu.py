@@ -590,6 +590,22 @@ def test_ops_refuse_mismatched_tensors():
             ops.cache_decode(_rows(2, heads, 1, 64, torch.bfloat16, 1).cuda(), cache, window=1, sink=1)
 
 
+@pytest.mark.parametrize("far", [101, 2 ** 31, 2 ** 32 + 5])
+def test_window_and_sink_beyond_the_cache(far):
+    """More than the cache holds means all keys, past 32 bits too; a negative one is refused."""
+    ops = _ops()
+    cache = _cache(1, 2, 100, 64, "e4m3", 32, seed=8)
+    x = _rows(1, 2, 100, 64, torch.bfloat16, 9).cuda()
+    ops.cache_write(cache, x, x, pos=0)
+    q = _rows(1, 4, 1, 64, torch.bfloat16, 10).cuda()
+    for kw in (dict(window=far, sink=0), dict(window=0, sink=far), dict(window=far, sink=far)):
+        _, sparse = ops.cache_decode(q, cache, want_dense=False, **kw)
+        _check_rows(sparse, q, cache, [100], kw["window"], kw["sink"], True, f"{kw}")
+    for kw in (dict(window=-far, sink=0), dict(window=0, sink=-far)):
+        with pytest.raises(ValueError, match="negative"):
+            ops.cache_decode(q, cache, **kw)
+
+
 def test_write_read_attend_together():
     """A prompt in chunks, then single tokens, as a decode loop runs them: the
     attention over the cache equals the dense path over what reads back, and
