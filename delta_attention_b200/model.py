@@ -205,6 +205,10 @@ class DeltaDecoder:
 
     def _attend(self, i: int, layer, q, k, v, prefill: bool, **kw) -> torch.Tensor:
         if self.attention is not None:
+            if isinstance(k, QuantizedKV):  # the override takes tensors
+                from . import ops
+
+                k, v = ops.cache_read(k, n_keys=kw["n_keys"], dtype=self.dtype)
             return self.attention(i, q, k, v, self.scaling, prefill)
         plug = layer["plugin"]
         if prefill:
@@ -433,10 +437,15 @@ class DecodeGraph:
                 self._step(anchor)
             self.graphs[anchor] = g
 
+    def _check_room(self) -> None:
+        if self.model.length >= self.model._capacity():
+            raise ValueError(f"KV cache is full ({self.model._capacity()} positions)")
+
     def start(self, first_token: torch.Tensor) -> None:
         """Begin decoding after :meth:`DeltaDecoder.prefill` (which returned
         ``first_token``): the next step writes cache position ``model.length``."""
         m = self.model
+        self._check_room()
         self.tok.copy_(first_token)
         self.pos.fill_(m.length)
         self.pos32.fill_(m.length)
@@ -448,6 +457,7 @@ class DecodeGraph:
     def step(self) -> torch.Tensor:
         """One token per sequence; returns the device tensor of the next token
         (overwritten by the next step)."""
+        self._check_room()
         anchor = self.mode == "delta" and self.steps % self.period == 0
         self.graphs[anchor].replay()
         self.steps += 1

@@ -134,6 +134,53 @@ def test_plugin_decode_policies_over_the_cache(policy):
     assert policy != "fixed" or len(a._dec_drift_points) == 16
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_attention_override_over_the_cache(fmt):
+    """An override gets the live keys and values as tensors, whatever the cache holds them as."""
+    from delta_attention_b200 import ops
+    m, plain = _decoder(fmt), _decoder(fmt)
+    seen = []
+
+    def attention(i, q, k, v, scaling, prefill):
+        seen.append((i, tuple(k.shape), k.dtype, prefill))
+        n, s = k.shape[2], q.shape[2]
+        rows = [orc.dense_decode(q[:, :, r:r + 1].float().cpu(), k[:, :, :n - s + 1 + r].float().cpu(),
+                                 v[:, :, :n - s + 1 + r].float().cpu(), scaling) for r in range(s)]
+        return torch.cat(rows, dim=1).to(q.dtype).to(q.device)
+
+    ids = _ids(2, SEQ + 9)
+    for x in (m, plain):
+        x.allocate_cache(2, SEQ + 32)
+        x.forward(ids[:, :SEQ])
+    m.attention = attention
+    at = SEQ
+    for n in (1, 7, 1):
+        _near(m.forward(ids[:, at:at + n]), plain.forward(ids[:, at:at + n]), f"{fmt} tokens [{at}, {at + n})")
+        at += n
+        assert seen[-2:] == [(i, (2, 2, at, 64), torch.bfloat16, False) for i in range(2)]
+    ops.check_errors()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_decode_graph_refuses_a_full_cache(fmt):
+    from delta_attention_b200 import ops
+    from delta_attention_b200.model import DecodeGraph
+    m = _decoder(fmt)
+    m.allocate_cache(1, 130)
+    tok = m.prefill(_ids(1, 128))
+    g = DecodeGraph(m, batch=1)
+    g.start(tok)
+    for _ in range(2):
+        g.step()
+    with pytest.raises(ValueError, match="full"):
+        g.step()
+    with pytest.raises(ValueError, match="full"):
+        g.start(tok)
+    assert m.length == 130
+    g.release()
+    ops.check_errors()
+
+
 def test_unknown_cache_format_is_refused():
     with pytest.raises(ValueError, match="kv_cache"):
         _decoder("fp4")
