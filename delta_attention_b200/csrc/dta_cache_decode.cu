@@ -106,8 +106,8 @@ struct MergeState {
     M = R = -INFINITY;
     L = 0.f;
   }
-  // Takes more chunks: wo their factors on o (0 for a chunk without keys); returns
-  // the factor that brings the o of earlier chunks to the new maximum.
+  // Takes more chunks: wo their factors on o (-1 for a chunk without keys, whose o was
+  // never written); returns the factor that brings the o of earlier chunks to the new maximum.
   __device__ __forceinline__ float weigh(const float (&m)[HEADS], const float (&l)[HEADS], const float (&r)[HEADS],
                                          float (&wo)[HEADS]) {
     float mt = M, rt = R;
@@ -125,7 +125,7 @@ struct MergeState {
 #pragma unroll
     for (int k = 0; k < HEADS; ++k) {
       sum += l[k] == 0.f ? 0.f : l[k] * fast_exp2(m[k] - mt);
-      wo[k] = l[k] == 0.f ? 0.f : fast_exp2(r[k] - rt);
+      wo[k] = l[k] == 0.f ? -1.f : fast_exp2(r[k] - rt);
     }
 #pragma unroll
     for (int x = 16; x > 0; x /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -139,7 +139,8 @@ struct MergeState {
     return __float2bfloat16_rn(L == 0.f ? 0.f : (o * 0x1p-14f) * exp2f(R - M) / L);
   }
 };
-__device__ __forceinline__ void merge_add(float& acc, float o, float w) { acc = w == 0.f ? acc : fmaf(o, w, acc); }
+// (A factor of 0 is applied: a chunk far below the maximum, or with no finite r, may hold a NaN, which stays.)
+__device__ __forceinline__ void merge_add(float& acc, float o, float w) { acc = w < 0.f ? acc : fmaf(o, w, acc); }
 constexpr int CD_CLUSTER_MAX = 16;  // CTAs of a cluster (above 8: non-portable sizes, used where they fit)
 
 // Shared-memory ring of one warp: CD_STAGES stages of CD_KEYS keys, each K rows
