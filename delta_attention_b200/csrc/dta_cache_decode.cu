@@ -13,9 +13,13 @@
 // by a power of two so that the largest element lies in [2^14, 2^15) (exact down to
 // 2^-29 of it); products and sums in fp32.  (The 8-bit mma.sync of this type converts
 // to fp16 itself: the kernel ran 25% more instructions with it.)  int8: codes as they
-// are, the query as a 16-bit integer, 32512 / max|q| times q (off by at most 1/65024 of
-// the largest element), in two 8-bit parts; products and sums in integers.  That costs no
-// conversion: 347 instructions for 16 keys, 364 to 398 with codes converted to fp16.
+// are, the queries times a power of two per head that brings the largest element to
+// [2^22, 2^23), as 24-bit integers in three 8-bit parts (bf16's bits are all kept down to
+// 2^-15 of the largest element, smaller ones are off by at most 2^-23 of it); products and
+// sums in integers.  With two parts (2^-16 of it) a query with one channel 200 times the
+// others was off by more than the output's rounding to bf16; the third part costs nothing at
+// d 128 (4 x 65536 keys, both rows: 87.9 us for 89.1) and 4% at 64 (4 x 131072: 98.1 for
+// 94.2).  With codes converted to fp16 the first of these took 102 us where two parts took 92.
 //
 // Split-K over the cache: CTA (chunk, batch x KV head) reads its chunk's codes once
 // for all G <= 8 query heads of the group; the partials (m, l, r, o) of the chunks
@@ -49,13 +53,22 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// A signed; B signed, or with `US` unsigned.
+template <bool US>
 __device__ __forceinline__ void mma_int8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (US)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Transposes an 8x8 matrix of 16-bit values held one row per lane quad.
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
@@ -274,8 +287,9 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
   }
 
   // ---- Q as the B operand: entry (c, i) holds head g's dims 16 (KP t + c) + 4 i + {0 .. 3}: as two
-  // fp16 pairs (e4m3), or their high and low bytes (int8) ----
-  uint32_t qb[KP][4][2];
+  // fp16 pairs (e4m3), or their high, middle and low bytes (int8) ----
+  constexpr int QW = FMT == CACHE_E4M3 ? 2 : 3;
+  uint32_t qb[KP][4][QW];
   float my_scale;
   {
     const bool hv = g < G;
@@ -295,16 +309,10 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       for (int e = 0; e < 8; ++e) top = max(top, max((w[c][e] << 16) & 0x7fffffffu, w[c][e] & 0x7fff0000u));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    float f;
-    if constexpr (FMT == CACHE_E4M3) {
-      const int up = min(max(141 - (int)(top >> 23), -126), 126);
-      f = __uint_as_float((uint32_t)(127 + up) << 23);
-      my_scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-    } else {
-      const float most = fmaxf(__uint_as_float(top), 0x1p-112f);  // (smaller heads would overflow f, and count as zeros)
-      f = 32512.f / most;
-      my_scale = p.scale_log2 * (most / 32512.f);
-    }
+    // the head's power of two: its largest element goes to [2^14, 2^15) (e4m3) or [2^22, 2^23) (int8)
+    const int up = min(max((FMT == CACHE_E4M3 ? 141 : 149) - (int)(top >> 23), -126), 126);
+    float f = __uint_as_float((uint32_t)(127 + up) << 23);
+    my_scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
     // a row with a non-finite element is NaN throughout
     if (top >= 0x7f800000u) {
       f = 0.f;
@@ -324,12 +332,13 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
           qb[c][i][0] = pack_f16x2(d[0], d[1]);
           qb[c][i][1] = pack_f16x2(d[2], d[3]);
         } else {
-          qb[c][i][0] = qb[c][i][1] = 0;
+          qb[c][i][0] = qb[c][i][1] = qb[c][i][2] = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int x = __float2int_rn(d[e]), hi = (x + 128) >> 8;  // |x| <= 32512, so |hi| <= 127
-            qb[c][i][0] |= (uint32_t)(hi & 255) << (8 * e);
-            qb[c][i][1] |= (uint32_t)(x & 255) << (8 * e);  // x - 256 hi, in [-128, 127]
+            const uint32_t x = (uint32_t)__float2int_rn(d[e]);  // |x| < 2^23: 2^16 (signed byte) + 2^8 byte + byte
+            qb[c][i][0] |= (x >> 16 & 255) << (8 * e);
+            qb[c][i][1] |= (x >> 8 & 255) << (8 * e);
+            qb[c][i][2] |= (x & 255) << (8 * e);
           }
         }
       }
@@ -379,7 +388,7 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
     float s[NG][4];
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
-      int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      int hi[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
       s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KP; ++c) {
@@ -395,14 +404,16 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
         } else {
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
-            mma_int8(hi, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][0], qb[c][i + 1][0]);
-            mma_int8(lo, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][1], qb[c][i + 1][1]);
+            mma_int8<false>(hi, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][0], qb[c][i + 1][0]);
+            mma_int8<true>(mid, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][1], qb[c][i + 1][1]);
+            mma_int8<true>(lo, w0[i], w1[i], w0[i + 1], w1[i + 1], qb[c][i][QW - 1], qb[c][i + 1][QW - 1]);
           }
         }
       }
       if constexpr (FMT == CACHE_INT8) {
+        // |hi| <= 2^21 is exact; |256 mid + lo| < 2^31 and its rounding is 2^-24 of it
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[q][e] = (float)(hi[e] * 256 + lo[e]);
+        for (int e = 0; e < 4; ++e) s[q][e] = fmaf((float)hi[e], 65536.f, (float)(mid[e] * 256 + lo[e]));
       }
     }
     // ---- weights ----

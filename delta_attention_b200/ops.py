@@ -594,7 +594,8 @@ def cache_decode(q: torch.Tensor, cache: QuantizedKV, *, window: int, sink: int,
                  n_keys_dev: Optional[torch.Tensor] = None,
                  ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """:func:`decode` over an 8-bit cache: one row per (batch, head), q [b, H, 1, d]
-    (computation from bf16 queries).  Returns ``(dense, sparse)``, each
+    (computation from bf16 queries; over an int8 cache an element below 2^-15 of its
+    row's largest magnitude is held to 2^-23 of that).  Returns ``(dense, sparse)``, each
     [b, 1, H, d] bf16 or None.  ``n_keys`` live keys (default: the capacity);
     ``n_keys_dev`` (device int32, 1 or b elements) gives the live counts on the
     device instead, at most ``n_keys``, which then sizes the launch.  A

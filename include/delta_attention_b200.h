@@ -337,7 +337,9 @@ DTA_API int dta_cache_read(const dta_cache_read_args* args, void* stream);
 
 /* dta_decode over an 8-bit cache: the dense and / or sparse row of every (batch,
  * head), same key sets.  q: [batch, n_heads, 1, head_dim] bf16; outputs
- * [batch, 1, n_heads, head_dim] bf16.  A sequence without keys gets zeros. */
+ * [batch, 1, n_heads, head_dim] bf16.  A sequence without keys gets zeros.  Over an
+ * int8 cache a query is held as 24-bit integers: an element below 2^-15 of its row's
+ * largest magnitude is off by at most 2^-23 of that. */
 typedef struct dta_cache_decode_args {
   int32_t abi_version;
   int32_t n_heads;
