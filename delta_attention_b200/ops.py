@@ -448,15 +448,20 @@ def _on_cache_device(op, cache, *args, **kw):
         return op(*args, **kw)
 
 
+def _torch_function(name: str, public):
+    """torch's private function ``name`` where it has one, else ``public``: these
+    ops run once per layer and token, and the public ones cost host time (a
+    Stream object 3 us, as much as launching a kernel)."""
+    return getattr(torch._C, name, None) or public
+
+
+_current_device = _torch_function("_cuda_getDevice", torch.cuda.current_device)
+# the current stream of a device, as an integer
+_raw_stream = _torch_function("_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _is_current(cache: QuantizedKV) -> bool:
-    return cache.index is not None and cache.index == torch._C._cuda_getDevice()
-
-
-def _raw_stream(index: int) -> int:
-    """The current stream of a device as an integer, without a Stream object:
-    these ops run once per layer and token, and building one costs as much
-    host time (3 us) as launching a kernel."""
-    return torch._C._cuda_getCurrentRawStream(index)
+    return cache.index is not None and cache.index == _current_device()
 
 
 _cache_ws = {}
@@ -467,7 +472,7 @@ def _cache_workspace(nbytes: int, index: int, stream: int):
     """(tensor, address, bytes), kept as :func:`_decode_workspace` keeps one.  The
     lock is held until the call's launches are queued: two host threads on one
     stream would otherwise interleave the launches of two calls that share it."""
-    capturing = torch._C._cuda_isCurrentStreamCapturing()
+    capturing = torch.cuda.is_current_stream_capturing()
     ws = None if capturing else _cache_ws.get((index, stream))
     if ws is None or ws[2] < nbytes:
         t = _workspace(nbytes, torch.device("cuda", index))
