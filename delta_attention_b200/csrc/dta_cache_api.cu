@@ -62,8 +62,11 @@ constexpr int kResidentCtas = 2;
 // resident with costs its own steps and kRampSteps; more of them the sum of their
 // costs over the slots and half a chunk's for the end; beyond 16 chunks per unit a
 // merge launch, two steps.  (128 + 2048 keys, 8 units: 6.0 us with 256-key chunks, 6.4 with
-// 384.)  It goes by sink, window, batch and heads only, so that a sparse row of a cache
-// is the same whichever call it comes from.
+// 384.)  It goes by the sink and window (each at most the call's n_keys), the units, the head
+// size and the device's SMs, not by the dense set or a device key count: on one device, calls
+// with the same n_keys cut a sparse row alike, with and without the dense one.  Calls
+// whose n_keys differ and lie below the sink or window may cut it differently (a host count,
+// and the capacity with that count on the device): those rows differ by rounding.
 constexpr int kSparseSteps[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32};
 constexpr int kSparseWaves = 4;  // chunks that would take more waves are not tried
 constexpr long long kSparseKeys = 1 << 23;  // windows beyond this take longer chunks (a launch has 65535 at most)

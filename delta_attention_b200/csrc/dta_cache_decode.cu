@@ -11,15 +11,17 @@
 //
 // The scores' operands.  e4m3: codes and queries in fp16, the queries scaled per head
 // by a power of two so that the largest element lies in [2^14, 2^15) (exact down to
-// 2^-29 of it); products and sums in fp32.  (The 8-bit mma.sync of this type converts
-// to fp16 itself: the kernel ran 25% more instructions with it.)  int8: codes as they
+// 2^-29 of it); products and sums in fp32.  (With the 8-bit mma.sync of this type the
+// kernel executed 25% more instructions.)  int8: codes as they
 // are, the queries times a power of two per head that brings the largest element to
 // [2^22, 2^23), as 24-bit integers in three 8-bit parts (bf16's bits are all kept down to
 // 2^-15 of the largest element, smaller ones are off by at most 2^-23 of it); products and
 // sums in integers.  With two parts (2^-16 of it) a query with one channel 200 times the
-// others was off by more than the output's rounding to bf16; the third part costs nothing at
-// d 128 (4 x 65536 keys, both rows: 87.9 us for 89.1) and 4% at 64 (4 x 131072: 98.1 for
-// 94.2).  With codes converted to fp16 the first of these took 102 us where two parts took 92.
+// others was off by more than the output's rounding to bf16.  The third costs 4% where calls
+// follow one another for long (4 x 65536 keys, both rows, d 128: 93.5 us for 90.0; dense, 4 x
+// 131072, d 64: 102.7 for 99.1), nothing at d 128 in short runs (87.9 for 89.1); four parts,
+// two to a product where a group has 4 heads at most, took as long.  With codes converted
+// to fp16 the first of these took 102 us where two parts took 92.
 //
 // Split-K over the cache: CTA (chunk, batch x KV head) reads its chunk's codes once
 // for all G <= 8 query heads of the group; the partials (m, l, r, o) of the chunks
@@ -193,12 +195,12 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&w)[2]) {
 // the sink and window in L2); its x the (batch, KV head) pairs.  CLU: the y extent is
 // one thread-block cluster per pair, and the cluster merges its chunks' partials through
 // distributed shared memory; else they go to global memory and cache_merge_kernel
-// merges them.  Both merge in one order, so a sparse row is the same bit for bit
-// whichever way it was launched.
+// merges them.  Both merge in one order, so calls with the same plan give the same row bit
+// for bit whichever way they merge.
 //
 // Why this shape.  At 8 bits a key costs half the memory time that it costs at 16, so
-// the instructions per key decide nearly as much as the memory does: 257 for 16 keys
-// (e4m3; 64 of them convert V and K), and the kernel without its copies takes 0.6 of
+// the instructions per key decide nearly as much as the memory does: 252 for 16 keys
+// (e4m3, 64 of them convert V and K; int8 368), and the kernel without its copies takes 0.6 of
 // the time of one without its products.  Hence rings per warp (no barrier in the loop),
 // 32 keys a step, maxima that move by vote, and two CTAs of 4 warps per SM with 16 KB per
 // warp on the way; 12 warps with 8 KB each, 16-key steps, and K and V in rings of their own
@@ -309,7 +311,8 @@ __global__ void __launch_bounds__(CD_THREADS) cache_decode_kernel(const __grid_c
       for (int e = 0; e < 8; ++e) top = max(top, max((w[c][e] << 16) & 0x7fffffffu, w[c][e] & 0x7fff0000u));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the head's power of two: its largest element goes to [2^14, 2^15) (e4m3) or [2^22, 2^23) (int8)
+    // the head's power of two: its largest element goes to [2^14, 2^15) (e4m3) or [2^22, 2^23) (int8;
+    // heads below 2^-104 keep fewer bits)
     const int up = min(max((FMT == CACHE_E4M3 ? 141 : 149) - (int)(top >> 23), -126), 126);
     float f = __uint_as_float((uint32_t)(127 + up) << 23);
     my_scale = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
