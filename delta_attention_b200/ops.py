@@ -511,8 +511,8 @@ def cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, *, pos, le
     kernel reads (a CUDA graph can then replay the call while the cache
     grows).  ``lengths`` (device int32, 1 or b elements): only the first
     ``lengths[i]`` rows of sequence i are written (a padded batch).  Rows
-    before ``pos`` keep their values (a block's scale only rises while it
-    holds earlier rows); rows behind the written ones are no longer live.
+    before ``pos`` stay (a block's scale only rises while it holds earlier rows,
+    whose codes are rounded to a raised one); rows behind the written ones are no longer live.
     A device position or length outside the cache writes nothing of that
     sequence and is recorded in the error word (:func:`check_errors`;
     ``check=True`` does that right after the launch)."""
